@@ -28,6 +28,48 @@ void launch_mse_bwd(const void* pred, const void* tgt, const float* gsum, size_t
 void launch_gather_rows(const void* x, const int* idx, int rows, int vec16_per_row, void* out, cudaStream_t s);
 int packed_ops_error_flag(bool reset);
 
+// ------------------------------------------------------------------ kept8_ops.cu, norm_ops.cu
+// Rows of a view with at most two strided leading levels (strides in elements, last dim adjacent).
+struct RowsArg {
+  const void* p;
+  long long outer_stride, inner_stride;
+  long long inner;  // rows of the inner level
+};
+// 8-bit kept rows of width C (layout in kept8.cuh); codes == nullptr: none.
+struct Kept8Buf {
+  void* codes;
+  void* scales;
+  int C;
+};
+void launch_keep8(const RowsArg& x, long long rows, bool fp32, const Kept8Buf& k, cudaStream_t s);
+// Rows row0 .. row0 + rows of `k` into out (row stride ld).
+void launch_restore8(const Kept8Buf& k, long long row0, long long rows, bool fp32, void* out, long long ld,
+                     cudaStream_t s);
+void launch_swiglu_fwd(const RowsArg& g, const RowsArg& v, long long rows, bool fp32, const Kept8Buf& kg,
+                       const Kept8Buf& kv, void* h, cudaStream_t s);
+void launch_swiglu_bwd(const RowsArg& dh, long long rows, bool fp32, const Kept8Buf& kg, const Kept8Buf& kv, void* dg,
+                       void* dv, void* h, cudaStream_t s);
+// part: fp32 [parts, C] scratch.
+int column_sum_parts(long long rows);
+void launch_column_sum(const RowsArg& x, long long rows, int C, bool fp32, float* part, int parts, void* out,
+                       bool out_fp32, cudaStream_t s);
+struct NormArgs {
+  long long rows;
+  int C;
+  bool fp32;       // x, y, dy, dx; bf16 otherwise
+  bool layer;      // layer norm; RMS norm otherwise
+  const void* w;   // [C] or null (ones)
+  const void* b;   // [C] or null (zeros)
+  bool w_fp32;     // w, b, dw, db
+  float eps;
+};
+// stats: fp32 [rows, 2] (mean, rstd) or null.
+void launch_norm_fwd(const NormArgs& a, const RowsArg& x, void* y, float* stats, const Kept8Buf& k, cudaStream_t s);
+// part: fp32 [parts, 2, C] scratch; dx, dw, db may be null.  x is read from `k` when that has codes.
+int norm_bwd_parts(const NormArgs& a);
+void launch_norm_bwd(const NormArgs& a, const RowsArg& dy, const RowsArg& x, const Kept8Buf& k, const float* stats,
+                     void* dx, float* part, int parts, void* dw, void* db, cudaStream_t s);
+
 // ------------------------------------------------------------------ gemm_sm100.cu
 constexpr int kGemmMaxGroups = 4;
 struct GemmGroup {

@@ -1,0 +1,108 @@
+"""Layer norm and RMS norm with learned weight and bias, as one autograd op each.
+
+``n = (x - mean) * rstd``, ``y = n * w + b`` (RMS norm: no mean, no bias), computed in fp32 and rounded
+once to ``x``'s dtype.  This is not the model's eager ``models.layers.rms_norm``, which also
+rounds ``n`` before the weight multiplies it.
+
+The backward returns ``dx`` and the fully reduced ``dw`` / ``db`` (fp32 sums in a fixed order: the same
+bits every time).  With ``kept8=True`` the input is kept in 8 bits (:mod:`pan2_b200.ops.kept8`) and the
+backward reads ``n`` from those, with the exact input's ``mean`` and ``rstd``.
+
+CUDA tensors (bf16 or fp32; any width, any leading dims, strided rows without a copy) run the
+sm_100a kernels of ``csrc/norm_ops.cu``; CPU tensors run plain PyTorch with the same math.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from ._ext import ext
+from .kept8 import _keep_cpu, _values_cpu, check_activation, wide_dtype
+
+
+class _Norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, eps, layer, kept8):
+        keep = kept8 and any(ctx.needs_input_grad[:2])
+        if x.is_cuda:
+            y, stats, codes, scales = ext().norm_fwd(x, w, b, eps, layer, keep)
+        else:
+            y, stats = _forward_cpu(x, w, b, eps, layer)
+            codes, scales = _keep_cpu(x) if keep else (None, None)
+        ctx.save_for_backward(None if keep else x, codes, scales, stats, w)
+        ctx.layer = layer
+        ctx.w_dtype = w.dtype if w is not None else b.dtype if b is not None else x.dtype
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, codes, scales, stats, w = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        if dy.is_cuda:
+            dx, dw, db = ext().norm_bwd(dy, x, codes, scales, stats, w, ctx.layer, need_x, need_w, need_b,
+                                        ctx.w_dtype == torch.float32)
+        else:
+            dx, dw, db = _backward_cpu(dy, x, codes, scales, stats, w, ctx.layer, ctx.w_dtype)
+        return dx if need_x else None, dw if need_w else None, db if need_b else None, None, None, None
+
+
+def _forward_cpu(x, w, b, eps, layer):
+    v = x.detach().to(wide_dtype(x.dtype))
+    mean = v.mean(-1, keepdim=True) if layer else v.new_zeros(*v.shape[:-1], 1)
+    rstd = torch.rsqrt((v - mean).square().mean(-1, keepdim=True) + eps)
+    y = (v - mean) * rstd
+    if w is not None:
+        y = y * w.to(y.dtype)
+    if b is not None:
+        y = y + b.to(y.dtype)
+    return y.to(x.dtype), torch.cat([mean, rstd], -1)
+
+
+def _backward_cpu(dy, x, codes, scales, stats, w, layer, w_dtype):
+    d = dy.to(wide_dtype(dy.dtype))
+    v = x.to(d.dtype) if codes is None else _values_cpu(codes, scales, dy.shape[-1], d.dtype).view(dy.shape)
+    mean, rstd = stats[..., :1], stats[..., 1:]
+    n = (v - mean) * rstd
+    g = d if w is None else d * w.to(d.dtype)
+    dx = g - n * (g * n).mean(-1, keepdim=True)
+    if layer:
+        dx = dx - g.mean(-1, keepdim=True)
+    rows = tuple(range(dy.dim() - 1))
+    total = (lambda t: t.sum(rows) if rows else t)
+    return (dx * rstd).to(dy.dtype), total(d * n).to(w_dtype), total(d).to(w_dtype)
+
+
+def _check(x, w, b, eps):
+    check_activation(x, "x")
+    for name, t in (("weight", w), ("bias", b)):
+        if t is None:
+            continue
+        if t.dim() != 1 or t.shape[0] != x.shape[-1]:
+            raise ValueError(f"{name} {tuple(t.shape)} does not fit rows of width {x.shape[-1]}")
+        if t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+        if x.is_cuda and t.dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError(f"{name} must be bf16 or fp32, got {t.dtype}")
+    if w is not None and b is not None and w.dtype != b.dtype:
+        raise TypeError(f"weight and bias have different dtypes: {w.dtype} and {b.dtype}")
+    if not eps >= 0:
+        raise ValueError(f"eps={eps} is negative")
+
+
+def _flat(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-6, kept8: bool = False) -> torch.Tensor:
+    """``(x - mean) * rsqrt(var + eps) * weight + bias`` over the last dim (biased variance)."""
+    _check(x, weight, bias, eps)
+    return _Norm.apply(x, _flat(weight), _flat(bias), float(eps), True, bool(kept8))
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+             kept8: bool = False) -> torch.Tensor:
+    """``x * rsqrt(mean(x^2) + eps) * weight`` over the last dim."""
+    _check(x, weight, None, eps)
+    return _Norm.apply(x, _flat(weight), None, float(eps), False, bool(kept8))
