@@ -426,10 +426,10 @@ std::vector<torch::Tensor> norm_bwd(torch::Tensor dy_, c10::optional<torch::Tens
   if (need_dx) dx = torch::empty(dy_.sizes(), dy.t.options());
   if (need_dw) dw = torch::empty({dy.C}, wopt);
   if (need_db) db = torch::empty({dy.C}, wopt);
-  const int parts = norm_bwd_parts(a);
-  if (need_dw || need_db) part = torch::empty({parts, 2, dy.C}, dy.t.options().dtype(torch::kFloat32));
+  if (need_dw || need_db)
+    part = torch::empty({norm_bwd_parts(a, dy.a, x.a, k), 2, dy.C}, dy.t.options().dtype(torch::kFloat32));
   launch_norm_bwd(a, dy.a, x.a, k, stats.data_ptr<float>(), need_dx ? dx.data_ptr() : nullptr,
-                  part.defined() ? part.data_ptr<float>() : nullptr, parts, need_dw ? dw.data_ptr() : nullptr,
+                  part.defined() ? part.data_ptr<float>() : nullptr, need_dw ? dw.data_ptr() : nullptr,
                   need_db ? db.data_ptr() : nullptr, stream());
   check_launch(nullptr, "norm_bwd");
   return {dx, dw, db};

@@ -137,22 +137,23 @@ __device__ __forceinline__ void kept8_store_codes(int8_t* p, const float (&v)[V]
   }
 }
 
+// Eight codes times their step.
+__device__ __forceinline__ void kept8_values(uint2 w, float step, float (&v)[8]) {
+  // byte k as an unsigned offset code in the mantissa of 2^23: 2^23 + (code + 128), exactly
+  const uint32_t u0 = w.x ^ 0x80808080u, u1 = w.y ^ 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = (__uint_as_float(__byte_perm(u0, 0x4b000000u, 0x7540 + i)) - 8388736.f) * step;
+    v[4 + i] = (__uint_as_float(__byte_perm(u1, 0x4b000000u, 0x7540 + i)) - 8388736.f) * step;
+  }
+}
+
 // V codes from `p` times the step of scale byte b.
 template <int V>
 __device__ __forceinline__ void kept8_load(const int8_t* p, uint32_t b, float (&v)[V]) {
   const float step = kept8_step(b);
-  if constexpr (V == 1) {
-    v[0] = (float)*p * step;
-  } else {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
-    // byte k of w as an unsigned offset code in the mantissa of 2^23: 2^23 + (code + 128), exactly
-    const uint32_t u0 = w.x ^ 0x80808080u, u1 = w.y ^ 0x80808080u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = (__uint_as_float(__byte_perm(u0, 0x4b000000u, 0x7540 + i)) - 8388736.f) * step;
-      v[4 + i] = (__uint_as_float(__byte_perm(u1, 0x4b000000u, 0x7540 + i)) - 8388736.f) * step;
-    }
-  }
+  if constexpr (V == 1) v[0] = (float)*p * step;
+  else kept8_values(*reinterpret_cast<const uint2*>(p), step, v);
 }
 
 // Scale byte of block `blk` of a row; the block's writer also fills the row's padding bytes.

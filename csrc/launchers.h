@@ -63,12 +63,13 @@ struct NormArgs {
   bool w_fp32;     // w, b, dw, db
   float eps;
 };
-// stats: fp32 [rows, 2] (mean, rstd) or null.
+// stats: fp32 [rows, 2] (mean, rstd).
 void launch_norm_fwd(const NormArgs& a, const RowsArg& x, void* y, float* stats, const Kept8Buf& k, cudaStream_t s);
-// part: fp32 [parts, 2, C] scratch; dx, dw, db may be null.  x is read from `k` when that has codes.
-int norm_bwd_parts(const NormArgs& a);
+// x is read from `k` when that has codes.  part: fp32 [norm_bwd_parts, 2, C] scratch, null when neither dw
+// nor db is wanted; dx, dw, db may be null.
+int norm_bwd_parts(const NormArgs& a, const RowsArg& dy, const RowsArg& x, const Kept8Buf& k);
 void launch_norm_bwd(const NormArgs& a, const RowsArg& dy, const RowsArg& x, const Kept8Buf& k, const float* stats,
-                     void* dx, float* part, int parts, void* dw, void* db, cudaStream_t s);
+                     void* dx, float* part, void* dw, void* db, cudaStream_t s);
 
 // ------------------------------------------------------------------ gemm_sm100.cu
 constexpr int kGemmMaxGroups = 4;
