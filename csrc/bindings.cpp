@@ -1,5 +1,5 @@
 // Python bindings of the sm_100a kernels: tensor validation, output allocation and stream
-// selection.  This is the only translation unit that includes torch headers.
+// selection.  Only this file and kept8_bindings.cpp include torch headers.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -30,6 +30,7 @@ const char* launch_attn_bwd(const void* q, const void* k, const void* v, const v
                             const float* lse, const int* items_q, int n_items_q, const int* items_kv, int n_items_kv,
                             int L, int H, int head_dim, float scale, float* delta, void* dq, void* dk, void* dv,
                             float* dq_acc, cudaStream_t s);
+void bind_kept8(pybind11::module_& m);  // kept8_bindings.cpp
 int attn_error_flag(bool reset);
 int qkv_bounds_error(bool reset);
 void attn_set_forward_variant(int v);
@@ -211,228 +212,6 @@ torch::Tensor gather_rows(torch::Tensor x, torch::Tensor idx) {
   launch_gather_rows(x.data_ptr(), idx.data_ptr<int>(), rows, (int)(row_bytes / 16), out.data_ptr(), stream());
   check_launch(nullptr, "gather_rows");
   return out;
-}
-
-// ---------------------------------------------------------------- 8-bit kept activations and norms
-namespace {
-
-// A tensor as rows of its last dimension; a copy is made only where the leading dimensions do not
-// collapse to two strided levels or the last dimension is not adjacent in memory.
-struct RowsOf {
-  torch::Tensor t;
-  RowsArg a;
-  int64_t rows;
-  int C;
-  bool fp32;
-};
-
-RowsOf rows_of(torch::Tensor t, const char* name) {
-  TORCH_CHECK(t.is_cuda() && (t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat32), name,
-              " must be a bf16 or fp32 CUDA tensor");
-  TORCH_CHECK(t.dim() >= 1 && t.size(-1) >= 1 && t.size(-1) < (1 << 30), name, " needs a last dimension of 1 .. 2^30");
-  if (t.size(-1) > 1 && t.stride(-1) != 1) t = t.contiguous();
-  RowsOf r;
-  r.C = (int)t.size(-1);
-  r.rows = t.numel() / r.C;
-  r.fp32 = t.scalar_type() == torch::kFloat32;
-  TORCH_CHECK(r.rows < (1ll << 31), name, " has 2^31 rows or more");
-  for (int attempt = 0;; ++attempt) {
-    int64_t size[2] = {1, 1}, stride[2] = {0, 0};  // inner, outer level
-    int levels = 0;
-    for (int64_t d = t.dim() - 2; d >= 0 && levels <= 2; --d) {
-      if (t.size(d) == 1) continue;
-      if (levels > 0 && t.stride(d) == size[levels - 1] * stride[levels - 1]) {
-        size[levels - 1] *= t.size(d);
-        continue;
-      }
-      if (levels < 2) {
-        size[levels] = t.size(d);
-        stride[levels] = t.stride(d);
-      }
-      ++levels;
-    }
-    if (levels <= 2 || attempt == 1) {
-      if (levels <= 1) r.a = RowsArg{t.data_ptr(), stride[0], 0, 1};
-      else r.a = RowsArg{t.data_ptr(), stride[1], stride[0], size[0]};
-      break;
-    }
-    t = t.contiguous();
-  }
-  if (r.a.inner < 1) r.a.inner = 1;  // no rows
-  r.t = t;
-  return r;
-}
-
-int64_t kept_width(int64_t C) { return (C + 31) / 32 * 32; }
-int64_t kept_scales(int64_t C) { return (kept_width(C) / 32 + 3) / 4 * 4; }
-
-Kept8Buf new_kept(const RowsOf& x, torch::Tensor& codes, torch::Tensor& scales) {
-  codes = torch::empty({x.rows, kept_width(x.C)}, x.t.options().dtype(torch::kInt8));
-  scales = torch::empty({x.rows, kept_scales(x.C)}, x.t.options().dtype(torch::kUInt8));
-  return Kept8Buf{codes.data_ptr(), scales.data_ptr(), x.C};
-}
-
-Kept8Buf kept_of(const torch::Tensor& codes, const torch::Tensor& scales, int64_t rows, int64_t C) {
-  TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == torch::kInt8 && codes.is_contiguous() && codes.dim() == 2 &&
-                  codes.size(0) == rows && codes.size(1) == kept_width(C),
-              "kept codes must be contiguous int8 [rows, C rounded up to 32]");
-  TORCH_CHECK(scales.is_cuda() && scales.scalar_type() == torch::kUInt8 && scales.is_contiguous() &&
-                  scales.dim() == 2 && scales.size(0) == rows && scales.size(1) == kept_scales(C) &&
-                  scales.device() == codes.device(),
-              "kept scales must be contiguous uint8 [rows, blocks rounded up to 4] beside the codes");
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0, "kept codes must be 16-byte aligned");
-  return Kept8Buf{codes.data_ptr(), scales.data_ptr(), (int)C};
-}
-
-void check_same(const RowsOf& a, const RowsOf& b, const char* what) {
-  TORCH_CHECK(a.rows == b.rows && a.C == b.C && a.fp32 == b.fp32 && a.t.device() == b.t.device(), what,
-              ": shapes, dtypes or devices differ");
-}
-
-NormArgs norm_args(const RowsOf& x, const c10::optional<torch::Tensor>& w, const c10::optional<torch::Tensor>& b,
-                   double eps, bool layer) {
-  NormArgs a{};
-  a.rows = x.rows;
-  a.C = x.C;
-  a.fp32 = x.fp32;
-  a.layer = layer;
-  a.eps = (float)eps;
-  a.w_fp32 = x.fp32;
-  const c10::optional<torch::Tensor>* vs[2] = {&w, &b};
-  const void** ps[2] = {&a.w, &a.b};
-  for (int i = 0; i < 2; ++i) {
-    if (!vs[i]->has_value()) continue;
-    const torch::Tensor& v = vs[i]->value();
-    TORCH_CHECK(v.dim() == 1 && v.size(0) == x.C && v.is_contiguous() && v.device() == x.t.device() &&
-                    (v.scalar_type() == torch::kFloat32 || v.scalar_type() == torch::kBFloat16),
-                "norm weight and bias must be contiguous bf16 or fp32 [C] tensors on x's device");
-    a.w_fp32 = v.scalar_type() == torch::kFloat32;
-    *ps[i] = v.data_ptr();
-  }
-  TORCH_CHECK(!w.has_value() || !b.has_value() || w->scalar_type() == b->scalar_type(),
-              "norm weight and bias must have one dtype");
-  return a;
-}
-
-}  // namespace
-
-std::vector<torch::Tensor> keep8(torch::Tensor x_) {
-  const at::cuda::CUDAGuard guard(x_.device());
-  const RowsOf x = rows_of(x_, "x");
-  torch::Tensor codes, scales;
-  const Kept8Buf k = new_kept(x, codes, scales);
-  launch_keep8(x.a, x.rows, x.fp32, k, stream());
-  check_launch(nullptr, "keep8");
-  return {codes, scales};
-}
-
-// Rows row0 .. row0 + out.size(0) of the kept tensor into `out` [rows, >= C], row-major.
-void restore8(torch::Tensor codes, torch::Tensor scales, int64_t C, int64_t row0, torch::Tensor out) {
-  const at::cuda::CUDAGuard guard(codes.device());
-  const Kept8Buf k = kept_of(codes, scales, codes.size(0), C);
-  TORCH_CHECK(out.is_cuda() && out.device() == codes.device() && out.dim() == 2 && out.size(1) >= C &&
-                  (out.size(1) == 1 || out.stride(1) == 1) &&
-                  (out.scalar_type() == torch::kBFloat16 || out.scalar_type() == torch::kFloat32),
-              "restore8: out must be a row-major bf16 or fp32 [rows, >= C] CUDA matrix");
-  TORCH_CHECK(row0 >= 0 && row0 + out.size(0) <= codes.size(0) && codes.size(0) < (1ll << 31),
-              "restore8: rows out of range");
-  launch_restore8(k, row0, out.size(0), out.scalar_type() == torch::kFloat32, out.data_ptr(), out.stride(0), stream());
-  check_launch(nullptr, "restore8");
-}
-
-// (h, codes and scales of gate, codes and scales of value)
-std::vector<torch::Tensor> swiglu8_fwd(torch::Tensor gate_, torch::Tensor value_) {
-  const at::cuda::CUDAGuard guard(gate_.device());
-  const RowsOf g = rows_of(gate_, "gate"), v = rows_of(value_, "value");
-  check_same(g, v, "gate and value");
-  auto h = torch::empty(gate_.sizes(), g.t.options());
-  torch::Tensor gc, gs, vc, vs;
-  const Kept8Buf kg = new_kept(g, gc, gs), kv = new_kept(v, vc, vs);
-  launch_swiglu_fwd(g.a, v.a, g.rows, g.fp32, kg, kv, h.data_ptr(), stream());
-  check_launch(nullptr, "swiglu8_fwd");
-  return {h, gc, gs, vc, vs};
-}
-
-// (dgate, dvalue[, h recomputed from the codes])
-std::vector<torch::Tensor> swiglu8_bwd(torch::Tensor dh_, torch::Tensor gc, torch::Tensor gs, torch::Tensor vc,
-                                       torch::Tensor vs, bool want_h) {
-  const at::cuda::CUDAGuard guard(dh_.device());
-  const RowsOf d = rows_of(dh_, "dh");
-  const Kept8Buf kg = kept_of(gc, gs, d.rows, d.C), kv = kept_of(vc, vs, d.rows, d.C);
-  TORCH_CHECK(gc.device() == dh_.device() && vc.device() == dh_.device(), "swiglu8_bwd: devices differ");
-  auto dg = torch::empty(dh_.sizes(), d.t.options()), dv = torch::empty(dh_.sizes(), d.t.options());
-  std::vector<torch::Tensor> out = {dg, dv};
-  if (want_h) out.push_back(torch::empty(dh_.sizes(), d.t.options()));
-  launch_swiglu_bwd(d.a, d.rows, d.fp32, kg, kv, dg.data_ptr(), dv.data_ptr(), want_h ? out[2].data_ptr() : nullptr,
-                    stream());
-  check_launch(nullptr, "swiglu8_bwd");
-  return out;
-}
-
-// Sum over rows in a fixed order, fp32 accumulation, in the dtype of x or fp32.
-torch::Tensor row_sum(torch::Tensor x_, bool fp32_out) {
-  const at::cuda::CUDAGuard guard(x_.device());
-  const RowsOf x = rows_of(x_, "x");
-  const int parts = column_sum_parts(x.rows);
-  auto part = torch::empty({parts, x.C}, x.t.options().dtype(torch::kFloat32));
-  auto out = torch::empty({x.C}, x.t.options().dtype(fp32_out ? torch::kFloat32 : x.t.scalar_type()));
-  launch_column_sum(x.a, x.rows, x.C, x.fp32, part.data_ptr<float>(), parts, out.data_ptr(),
-                    out.scalar_type() == torch::kFloat32, stream());
-  check_launch(nullptr, "row_sum");
-  return out;
-}
-
-// (y, stats, codes, scales); codes and scales are empty unless `kept`.
-std::vector<torch::Tensor> norm_fwd(torch::Tensor x_, c10::optional<torch::Tensor> w, c10::optional<torch::Tensor> b,
-                                    double eps, bool layer, bool kept) {
-  const at::cuda::CUDAGuard guard(x_.device());
-  const RowsOf x = rows_of(x_, "x");
-  const NormArgs a = norm_args(x, w, b, eps, layer);
-  auto y = torch::empty(x_.sizes(), x.t.options());
-  auto stats = torch::empty({x.rows, 2}, x.t.options().dtype(torch::kFloat32));
-  torch::Tensor codes, scales;
-  Kept8Buf k{nullptr, nullptr, x.C};
-  if (kept) k = new_kept(x, codes, scales);
-  launch_norm_fwd(a, x.a, y.data_ptr(), stats.data_ptr<float>(), k, stream());
-  check_launch(nullptr, "norm_fwd");
-  return {y, stats, codes, scales};
-}
-
-// (dx, dw, db); what is not asked for is an undefined tensor.  x: the tensor, or (codes, scales).
-std::vector<torch::Tensor> norm_bwd(torch::Tensor dy_, c10::optional<torch::Tensor> x_,
-                                    c10::optional<torch::Tensor> codes, c10::optional<torch::Tensor> scales,
-                                    torch::Tensor stats, c10::optional<torch::Tensor> w, bool layer, bool need_dx,
-                                    bool need_dw, bool need_db, bool w_fp32) {
-  const at::cuda::CUDAGuard guard(dy_.device());
-  const RowsOf dy = rows_of(dy_, "dy");
-  NormArgs a = norm_args(dy, w, c10::nullopt, 0.0, layer);
-  a.w_fp32 = w_fp32;
-  TORCH_CHECK(!w.has_value() || (w->scalar_type() == torch::kFloat32) == w_fp32, "norm_bwd: weight dtype");
-  TORCH_CHECK(stats.is_cuda() && stats.device() == dy_.device() && stats.scalar_type() == torch::kFloat32 &&
-                  stats.is_contiguous() && stats.numel() == 2 * dy.rows,
-              "norm_bwd: stats must be fp32 [rows, 2]");
-  RowsOf x = dy;
-  Kept8Buf k{nullptr, nullptr, dy.C};
-  if (codes.has_value()) {
-    TORCH_CHECK(scales.has_value() && codes->device() == dy_.device(), "norm_bwd: codes without scales, or elsewhere");
-    k = kept_of(*codes, *scales, dy.rows, dy.C);
-  } else {
-    TORCH_CHECK(x_.has_value(), "norm_bwd: x or its codes");
-    x = rows_of(*x_, "x");
-    check_same(dy, x, "dy and x");
-  }
-  torch::Tensor dx, dw, db, part;
-  const auto wopt = dy.t.options().dtype(w_fp32 ? torch::kFloat32 : torch::kBFloat16);
-  if (need_dx) dx = torch::empty(dy_.sizes(), dy.t.options());
-  if (need_dw) dw = torch::empty({dy.C}, wopt);
-  if (need_db) db = torch::empty({dy.C}, wopt);
-  if (need_dw || need_db)
-    part = torch::empty({norm_bwd_parts(a, dy.a, x.a, k), 2, dy.C}, dy.t.options().dtype(torch::kFloat32));
-  launch_norm_bwd(a, dy.a, x.a, k, stats.data_ptr<float>(), need_dx ? dx.data_ptr() : nullptr,
-                  part.defined() ? part.data_ptr<float>() : nullptr, need_dw ? dw.data_ptr() : nullptr,
-                  need_db ? db.data_ptr() : nullptr, stream());
-  check_launch(nullptr, "norm_bwd");
-  return {dx, dw, db};
 }
 
 // ------------------------------------------------------------------ GEMM
@@ -977,13 +756,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mse_fwd", &pan::mse_fwd, kNoGil);
   m.def("mse_bwd", &pan::mse_bwd, kNoGil);
   m.def("gather_rows", &pan::gather_rows, kNoGil);
-  m.def("keep8", &pan::keep8, kNoGil);
-  m.def("restore8", &pan::restore8, kNoGil);
-  m.def("swiglu8_fwd", &pan::swiglu8_fwd, kNoGil);
-  m.def("swiglu8_bwd", &pan::swiglu8_bwd, kNoGil);
-  m.def("row_sum", &pan::row_sum, kNoGil);
-  m.def("norm_fwd", &pan::norm_fwd, kNoGil);
-  m.def("norm_bwd", &pan::norm_bwd, kNoGil);
+  pan::bind_kept8(m);
   m.def("gemm", &pan::gemm, kNoGil);
   m.def("gemm_force_cta_group", &pan::gemm_force_cta_group, kNoGil);
   m.def("attn_set_forward_variant", &pan::attn_set_forward_variant, kNoGil);

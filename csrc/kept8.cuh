@@ -87,6 +87,70 @@ __device__ __forceinline__ void store_v(T* p, const float (&v)[V]) {
   }
 }
 
+// ---------------------------------------------------------------- packed fp32 pairs
+// Two fp32 operations an instruction: these kernels are as often bound by instruction issue as by DRAM.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mov.b64 rc, {%6, %7};\n\tfma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
+
+// Eight consecutive elements as they lie in memory, and as fp32 pairs.
+template <typename T>
+struct Frag;
+template <>
+struct Frag<__nv_bfloat16> {
+  uint4 raw;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { raw = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float2 (&v)[4]) const {
+    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+  }
+};
+template <>
+struct Frag<float> {
+  float4 raw[2];
+  __device__ __forceinline__ void load(const float* p) {
+    raw[0] = reinterpret_cast<const float4*>(p)[0];
+    raw[1] = reinterpret_cast<const float4*>(p)[1];
+  }
+  __device__ __forceinline__ void zero() { raw[0] = raw[1] = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void get(float2 (&v)[4]) const {
+    v[0] = make_float2(raw[0].x, raw[0].y);
+    v[1] = make_float2(raw[0].z, raw[0].w);
+    v[2] = make_float2(raw[1].x, raw[1].y);
+    v[3] = make_float2(raw[1].z, raw[1].w);
+  }
+};
+
+__device__ __forceinline__ void store_pairs(__nv_bfloat16* p, const float2 (&v)[4]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(v[0].x, v[0].y), pack_bf16(v[1].x, v[1].y),
+                                            pack_bf16(v[2].x, v[2].y), pack_bf16(v[3].x, v[3].y));
+}
+__device__ __forceinline__ void store_pairs(float* p, const float2 (&v)[4]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+}
+
 // ---------------------------------------------------------------- codes
 // Scale byte from the bits of max |x|.  NaN has the largest bits, then Inf: both give 255.
 __device__ __forceinline__ uint32_t kept8_byte(uint32_t amax_bits) { return max(amax_bits >> 23, 7u); }
@@ -137,23 +201,81 @@ __device__ __forceinline__ void kept8_store_codes(int8_t* p, const float (&v)[V]
   }
 }
 
-// Eight codes times their step.
-__device__ __forceinline__ void kept8_values(uint2 w, float step, float (&v)[8]) {
+// Eight codes as numbers.
+__device__ __forceinline__ void kept8_numbers(uint2 w, float2 (&v)[4]) {
   // byte k as an unsigned offset code in the mantissa of 2^23: 2^23 + (code + 128), exactly
-  const uint32_t u0 = w.x ^ 0x80808080u, u1 = w.y ^ 0x80808080u;
+  const uint32_t u[2] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    v[i] = (__uint_as_float(__byte_perm(u0, 0x4b000000u, 0x7540 + i)) - 8388736.f) * step;
-    v[4 + i] = (__uint_as_float(__byte_perm(u1, 0x4b000000u, 0x7540 + i)) - 8388736.f) * step;
+    const float2 m = make_float2(__uint_as_float(__byte_perm(u[i / 2], 0x4b000000u, 0x7540 + i % 2 * 2)),
+                                 __uint_as_float(__byte_perm(u[i / 2], 0x4b000000u, 0x7541 + i % 2 * 2)));
+    v[i] = add2(m, twice(-8388736.f));
   }
+}
+__device__ __forceinline__ float kept8_number(int8_t code) {
+  return __uint_as_float(((uint8_t)code ^ 0x80u) | 0x4b000000u) - 8388736.f;
+}
+// ... times their step.
+__device__ __forceinline__ void kept8_values(uint2 w, float step, float2 (&v)[4]) {
+  kept8_numbers(w, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], twice(step));
+}
+__device__ __forceinline__ void kept8_values(uint2 w, float step, float (&v)[8]) {
+  float2 p[4];
+  kept8_values(w, step, p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[2 * i] = p[i].x, v[2 * i + 1] = p[i].y;
 }
 
 // V codes from `p` times the step of scale byte b.
 template <int V>
 __device__ __forceinline__ void kept8_load(const int8_t* p, uint32_t b, float (&v)[V]) {
   const float step = kept8_step(b);
-  if constexpr (V == 1) v[0] = (float)*p * step;
+  if constexpr (V == 1) v[0] = kept8_number(*p) * step;
   else kept8_values(*reinterpret_cast<const uint2*>(p), step, v);
+}
+
+// Scale byte and codes of a fragment whose block is held by four neighbouring lanes; every lane of the
+// warp takes part.
+__device__ __forceinline__ void kept8_encode(const Frag<float>& f, uint32_t& b, uint2& codes) {
+  const float v[8] = {f.raw[0].x, f.raw[0].y, f.raw[0].z, f.raw[0].w, f.raw[1].x, f.raw[1].y, f.raw[1].z, f.raw[1].w};
+  b = kept8_byte(kept8_amax<8>(v));
+  const float inv = kept8_inv_step(b);
+  uint32_t c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = kept8_code(v[i], inv);
+  codes = make_uint2(pack4_low_bytes(c[0], c[1], c[2], c[3]), pack4_low_bytes(c[4], c[5], c[6], c[7]));
+}
+
+// In bf16 pairs: |x| is clamped to 127 steps, and one fused multiply-add |x| / step + 128 rounds it half to
+// even to a whole number whose low seven mantissa bits are the magnitude (128 .. 255 has a unit of 1 in
+// bf16).  Four magnitudes a word then take their signs as bytes: -m = (0x80 - m) ^ 0x80 without borrows.
+__device__ __forceinline__ void kept8_encode(const Frag<__nv_bfloat16>& f, uint32_t& b, uint2& codes) {
+  const uint32_t w[4] = {f.raw.x, f.raw.y, f.raw.z, f.raw.w};
+  uint32_t a[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i] = w[i] & 0x7fff7fffu;
+  uint32_t m = __vmaxu2(__vmaxu2(a[0], a[1]), __vmaxu2(a[2], a[3]));
+  m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  b = max(max(m & 0xffffu, m >> 16) >> 7, 7u);
+  const uint32_t lim = ((b << 7) | 0x7eu) * 0x10001u;  // 127 steps
+  const uint32_t inv = ((260u - b) << 7) * 0x10001u;
+  uint32_t z[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    asm("{\n\t.reg .b32 t;\n\tmin.bf16x2 t, %1, %2;\n\tfma.rn.bf16x2 %0, t, %3, %4;\n\t}"
+        : "=r"(z[i]) : "r"(a[i]), "r"(lim), "r"(inv), "r"(0x43004300u));
+  uint32_t c[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t mag = __byte_perm(z[2 * i], z[2 * i + 1], 0x6420);
+    uint32_t neg;  // 0xff where the element's sign bit is set
+    asm("prmt.b32 %0, %1, %2, 0xfdb9;" : "=r"(neg) : "r"(w[2 * i]), "r"(w[2 * i + 1]));
+    c[i] = ((0x80808080u - (mag & neg)) ^ 0x80808080u) | (mag & ~neg);
+  }
+  codes = make_uint2(c[0], c[1]);
 }
 
 // Scale byte of block `blk` of a row; the block's writer also fills the row's padding bytes.

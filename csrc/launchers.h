@@ -1,7 +1,7 @@
 // Plain-C++ launch interface of the sm_100a kernels.  The .cu files implement these with raw
-// pointers and a CUDA stream; bindings.cpp (the only file that includes torch headers) validates
-// tensors, allocates outputs and calls them.  Keeping torch out of nvcc's translation units keeps
-// kernel rebuilds to seconds.
+// pointers and a CUDA stream; the bindings (bindings.cpp and kept8_bindings.cpp, the only files that
+// include torch headers) validate tensors, allocate outputs and call them.  Keeping torch out of
+// nvcc's translation units keeps kernel rebuilds to seconds.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -41,7 +41,11 @@ struct Kept8Buf {
   void* scales;
   int C;
 };
-void launch_keep8(const RowsArg& x, long long rows, bool fp32, const Kept8Buf& k, cudaStream_t s);
+// copy (bf16 x only, may be null): x itself with row stride ld, ld / 8 whole, zeros past C.
+void launch_keep8(const RowsArg& x, long long rows, bool fp32, const Kept8Buf& k, void* copy, long long ld,
+                  cudaStream_t s);
+// out [rows, ld] bf16 = x [rows, C], zeros past C (ld = C rounded up to 8).
+void launch_pad_rows(const RowsArg& x, long long rows, int C, void* out, long long ld, cudaStream_t s);
 // Rows row0 .. row0 + rows of `k` into out (row stride ld).
 void launch_restore8(const Kept8Buf& k, long long row0, long long rows, bool fp32, void* out, long long ld,
                      cudaStream_t s);
@@ -49,8 +53,8 @@ void launch_swiglu_fwd(const RowsArg& g, const RowsArg& v, long long rows, bool 
                        const Kept8Buf& kv, void* h, cudaStream_t s);
 void launch_swiglu_bwd(const RowsArg& dh, long long rows, bool fp32, const Kept8Buf& kg, const Kept8Buf& kv, void* dg,
                        void* dv, void* h, cudaStream_t s);
-// part: fp32 [parts, C] scratch.
-int column_sum_parts(long long rows);
+// part: fp32 [parts, C] scratch (unused when parts == 1).
+int column_sum_parts(long long rows, int C);
 void launch_column_sum(const RowsArg& x, long long rows, int C, bool fp32, float* part, int parts, void* out,
                        bool out_fp32, cudaStream_t s);
 struct NormArgs {
@@ -63,7 +67,7 @@ struct NormArgs {
   bool w_fp32;     // w, b, dw, db
   float eps;
 };
-// stats: fp32 [rows, 2] (mean, rstd).
+// stats: fp32 [rows, 2] (mean, rstd) or null.
 void launch_norm_fwd(const NormArgs& a, const RowsArg& x, void* y, float* stats, const Kept8Buf& k, cudaStream_t s);
 // x is read from `k` when that has codes.  part: fp32 [norm_bwd_parts, 2, C] scratch, null when neither dw
 // nor db is wanted; dx, dw, db may be null.

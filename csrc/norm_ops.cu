@@ -8,14 +8,14 @@
 // does not cancel the variance away.  The backward reads x either as it was or from its 8-bit codes
 // (kept8.cuh); mean and rstd are always those of the exact x.
 //
-// Both directions are DRAM-bound, so every tensor is read and written once.  A group of G threads
-// holds a whole row in registers in fragments of V elements (V = 8: 16-byte accesses, for rows whose
-// width and alignment allow; V = 1 otherwise; fragment i of thread t starts at column (t + i G) V).
-// Groups of up to a warp reduce by shuffles, larger ones through shared memory.  The
-// backward's threads own their columns for all the rows that their CTA walks, so dw and db grow in
-// registers beside the dx of each row; one partial row per CTA goes to scratch and a second kernel adds those up
-// in order (no atomics: the same bits every time).  Rows too wide for registers take the *_wide
-// kernels, which sweep the row from memory.
+// Both directions are DRAM-bound, so every tensor is read and written once.  A group of G threads owns the
+// columns of a row for all the rows that its CTA walks: weight, bias and the growing dw / db stay in
+// registers, and one partial row of dw / db per CTA goes to scratch, which a second kernel adds up in order (no
+// atomics: the same bits every time).  Three forms:
+//   staged   (C % 8 == 0, 16-byte aligned rows, C <= 16384)  8-column fragments through rings in shared memory
+//   single   (any other rows up to 16384 / 8192 columns)     one column at a time, rows in registers
+//   wide     (wider rows)                                    CTA per row, the row swept from memory
+// Groups of up to a warp reduce by shuffles, larger ones through shared memory.
 #include "kept8.cuh"
 #include "launchers.h"
 
@@ -23,6 +23,7 @@ namespace pan {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int threads_of(int G) { return G > kThreads ? G : kThreads; }
 
 struct Kept {
   int8_t* codes;
@@ -36,61 +37,6 @@ struct Vectors {  // learned weight and bias, bf16 or fp32, either may be missin
   bool fp32;
 };
 
-// ---------------------------------------------------------------- fragments
-// V elements as they lie in memory.
-template <typename T, int V>
-struct Pack {
-  T raw;
-  __device__ __forceinline__ void load(const T* p) { raw = *p; }
-  __device__ __forceinline__ void zero() { raw = from_f32<T>(0.f); }
-  __device__ __forceinline__ void get(float (&v)[V]) const { v[0] = to_f32(raw); }
-};
-template <>
-struct Pack<__nv_bfloat16, 8> {
-  uint4 raw;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { raw = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(u[i] << 16);
-      v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    }
-  }
-};
-template <>
-struct Pack<float, 8> {
-  float4 raw[2];
-  __device__ __forceinline__ void load(const float* p) {
-    raw[0] = reinterpret_cast<const float4*>(p)[0];
-    raw[1] = reinterpret_cast<const float4*>(p)[1];
-  }
-  __device__ __forceinline__ void zero() { raw[0] = raw[1] = make_float4(0.f, 0.f, 0.f, 0.f); }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-    v[0] = raw[0].x; v[1] = raw[0].y; v[2] = raw[0].z; v[3] = raw[0].w;
-    v[4] = raw[1].x; v[5] = raw[1].y; v[6] = raw[1].z; v[7] = raw[1].w;
-  }
-};
-
-// V codes and their scale byte.
-template <int V>
-struct CodePack {
-  uint2 raw;
-  uint32_t b;
-  __device__ __forceinline__ void load(const int8_t* p, uint32_t byte) {
-    if constexpr (V == 8) raw = *reinterpret_cast<const uint2*>(p);
-    else raw.x = (uint8_t)*p;
-    b = byte;
-  }
-  __device__ __forceinline__ void zero() { raw = make_uint2(0, 0), b = kKeptPadByte; }
-  __device__ __forceinline__ void get(float (&v)[V]) const {
-    const float step = kept8_step(b);
-    if constexpr (V == 8) kept8_values(raw, step, v);
-    else v[0] = (float)(int8_t)raw.x * step;
-  }
-};
-
 template <int V>
 __device__ __forceinline__ void load_vec(const void* p, bool fp32, int c, float missing, float (&v)[V]) {
   if (p == nullptr) {
@@ -101,6 +47,25 @@ __device__ __forceinline__ void load_vec(const void* p, bool fp32, int c, float 
   } else {
     load_v<__nv_bfloat16, V>(reinterpret_cast<const __nv_bfloat16*>(p) + c, v);
   }
+}
+
+__device__ __forceinline__ float vec_at(const void* p, bool fp32, int c, float missing) {
+  float v[1];
+  load_vec<1>(p, fp32, c, missing, v);
+  return v[0];
+}
+
+// Eight columns from c on, `missing` past the row's end.
+__device__ __forceinline__ void load_pairs(const void* p, bool fp32, int c, int C, float missing, float2 (&v)[4]) {
+  float f[8];
+  load_vec<8>(c < C ? p : nullptr, fp32, c, missing, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = make_float2(f[2 * i], f[2 * i + 1]);
+}
+
+template <typename W>
+__device__ __forceinline__ void store_out(void* out, int c, float v) {
+  if (out != nullptr) reinterpret_cast<W*>(out)[c] = from_f32<W>(v);
 }
 
 // ---------------------------------------------------------------- reductions
@@ -130,396 +95,324 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float* ws) {
   }
 }
 
-// ---------------------------------------------------------------- forward
-// The row lives in registers between its one read and its one write, so the mean, the centred squares, the
-// codes and y all come from it.  Up to a warp a row needs no barrier and several rows are in flight a CTA.
-template <typename T, int V, int G, int UPT>
-__global__ void __launch_bounds__(G > kThreads ? G : kThreads)
-    norm_fwd_kernel(RowView x, uint32_t rows, int C, Vectors vec, float eps, bool layer, T* __restrict__ y,
-                    float* __restrict__ stats, Kept k) {
-  constexpr int NT = G > kThreads ? G : kThreads, GROUPS = NT / G;
-  __shared__ float ws[2][NT / 32];
-  const int t = threadIdx.x % G;
-  const uint32_t r = blockIdx.x * GROUPS + threadIdx.x / G;
-  const bool in = r < rows;
-  const T* xr = row_ptr<T>(x, in ? r : 0);
-  Pack<T, V> raw[UPT];
-#pragma unroll
-  for (int i = 0; i < UPT; ++i) {
-    const int c = (t + i * G) * V;
-    if (in && c < C) raw[i].load(xr + c);
-    else raw[i].zero();
-  }
-  float mean = 0.f;
-  const float inv_c = 1.f / C;
-  if (layer) {
-    float s[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < UPT; ++i) {
-      float v[V];
-      raw[i].get(v);
-#pragma unroll
-      for (int j = 0; j < V; ++j) s[0] += v[j];
-    }
-    group_sum<G, 1>(s, ws[0]);
-    mean = s[0] * inv_c;
-  }
-  float s[1] = {0.f};
-#pragma unroll
-  for (int i = 0; i < UPT; ++i) {
-    if ((t + i * G) * V >= C) continue;
-    float v[V];
-    raw[i].get(v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) s[0] += (v[j] - mean) * (v[j] - mean);
-  }
-  group_sum<G, 1>(s, ws[1]);
-  const float rstd = rsqrtf(s[0] * inv_c + eps);
-  if (in && t == 0) *reinterpret_cast<float2*>(stats + 2 * (size_t)r) = make_float2(mean, rstd);
-  T* yr = y + (long long)r * C;
-#pragma unroll
-  for (int i = 0; i < UPT; ++i) {
-    const int c = (t + i * G) * V;
-    float v[V];
-    raw[i].get(v);
-    if (k.codes != nullptr) {  // whole blocks of 32 / V neighbouring lanes, with zeros past the row's end
-      const uint32_t b = kept8_byte(kept8_amax<V>(v));
-      if (in && c < k.Cp) {
-        kept8_store_codes<V>(k.codes + (long long)r * k.Cp + c, v, b);
-        if (c % kKeptBlock == 0) kept8_store_byte(k.scales + (long long)r * k.nbp, c / kKeptBlock, k.nb, k.nbp, b);
-      }
-    }
-    if (!in || c >= C) continue;
-    float w[V], b[V];
-    load_vec<V>(vec.w, vec.fp32, c, 1.f, w);
-    load_vec<V>(vec.b, vec.fp32, c, 0.f, b);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = (v[j] - mean) * rstd * w[j] + b[j];
-    store_v<T, V>(yr + c, v);
-  }
-}
-
-// ---------------------------------------------------------------- backward
-// x of a fragment comes from the tensor or from the codes (KEPT).
-template <typename T, int V, bool KEPT>
-struct XPack : Pack<T, V> {
-  __device__ __forceinline__ void load(const RowView& x, const Kept&, uint32_t r, int c) {
-    Pack<T, V>::load(row_ptr<T>(x, r) + c);
-  }
-};
-template <typename T, int V>
-struct XPack<T, V, true> : CodePack<V> {
-  __device__ __forceinline__ void load(const RowView&, const Kept& k, uint32_t r, int c) {
-    CodePack<V>::load(k.codes + (long long)r * k.Cp + c, k.scales[(long long)r * k.nbp + c / kKeptBlock]);
-  }
-};
-
-template <typename W>
-__device__ __forceinline__ void store_out(void* out, int c, float v) {
-  if (out != nullptr) reinterpret_cast<W*>(out)[c] = from_f32<W>(v);
-}
-
-// The CTA's groups hold the same columns: add them up, in a fixed order, into the first group.
-template <int V, int G, int GROUPS, int UPT, bool BOTH>
-__device__ __forceinline__ void join_groups(float* aw, float* ab, int t, int group) {
-  if constexpr (GROUPS > 1) {
-    __shared__ float cs[GROUPS / 2 * G * V];
-#pragma unroll
-    for (int i = 0; i < UPT; ++i) {
-#pragma unroll
-      for (int which = 0; which < (BOTH ? 2 : 1); ++which) {
-        float* acc = (which ? ab : aw) + i * V;
-#pragma unroll
-        for (int h = GROUPS / 2; h > 0; h >>= 1) {
-          __syncthreads();
-          if (group >= h && group < 2 * h) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) cs[((group - h) * V + j) * G + t] = acc[j];
-          }
-          __syncthreads();
-          if (group < h) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] += cs[(group * V + j) * G + t];
-          }
-        }
-      }
-    }
-  }
-}
-
-// The CTA's partial row; a lone CTA's is the result.
-template <int V, int G, int UPT, bool BOTH>
-__device__ __forceinline__ void store_partial(const float* aw, const float* ab, int t, int C, bool fp32, float* part,
-                                              void* dw, void* db) {
-#pragma unroll
-  for (int i = 0; i < UPT; ++i) {
-    const int c = (t + i * G) * V;
-    if (c >= C) continue;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      if (gridDim.x == 1) {
-        if (fp32) store_out<float>(dw, c + j, aw[i * V + j]);
-        else store_out<__nv_bfloat16>(dw, c + j, aw[i * V + j]);
-        if (BOTH && fp32) store_out<float>(db, c + j, ab[i * V + j]);
-        else if (BOTH) store_out<__nv_bfloat16>(db, c + j, ab[i * V + j]);
-      } else {
-        part[(long long)blockIdx.x * 2 * C + c + j] = aw[i * V + j];
-        if (BOTH) part[((long long)blockIdx.x * 2 + 1) * C + c + j] = ab[i * V + j];
-      }
-    }
-  }
-}
-
-// ---- register form (rows that 16-byte copies cannot address): R rows a group at a time, all their loads issued
-// before the first reduction
-template <typename T, int V, int G, int UPT, int R, bool KEPT>
-__global__ void __launch_bounds__(G > kThreads ? G : kThreads, G > kThreads ? 1 : 2)
-    norm_bwd_kernel(RowView dy, RowView x, Kept k, uint32_t rows, int C, Vectors vec, bool layer,
-                    const float* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, void* dw, void* db) {
-  constexpr int NT = G > kThreads ? G : kThreads, GROUPS = NT / G, E = UPT * V;
-  __shared__ float ws[2][NT / 32 * 2 * R];
-  const int t = threadIdx.x % G, group = threadIdx.x / G;
-  float w[E], aw[E], ab[E];
-#pragma unroll
-  for (int i = 0; i < UPT; ++i) {
-    float v[V];
-    const int c = (t + i * G) * V;
-    load_vec<V>(c < C ? vec.w : nullptr, vec.fp32, c, 1.f, v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) w[i * V + j] = v[j], aw[i * V + j] = ab[i * V + j] = 0.f;
-  }
-  const float inv_c = 1.f / C;
-  int flip = 0;
-  for (uint32_t r0 = blockIdx.x * (GROUPS * R); r0 < rows; r0 += gridDim.x * (GROUPS * R)) {
-    Pack<T, V> gp[R][UPT];
-    XPack<T, V, KEPT> xp[R][UPT];
-    float2 st[R];
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      const uint32_t r = r0 + q * GROUPS + group;
-      const bool in = r < rows;
-      const T* gr = row_ptr<T>(dy, in ? r : 0);
-      st[q] = in ? *reinterpret_cast<const float2*>(stats + 2 * (size_t)r) : make_float2(0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-        const int c = (t + i * G) * V;
-        if (in && c < C) {
-          gp[q][i].load(gr + c);
-          xp[q][i].load(x, k, r, c);
-        } else {
-          gp[q][i].zero();
-          xp[q][i].zero();
-        }
-      }
-    }
-    float s[2 * R];
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      s[2 * q] = s[2 * q + 1] = 0.f;
-#pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-        float g[V], v[V];
-        gp[q][i].get(g);
-        xp[q][i].get(v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float n = (v[j] - st[q].x) * st[q].y;
-          const float gw = g[j] * w[i * V + j];
-          s[2 * q] += gw;
-          s[2 * q + 1] += gw * n;
-          aw[i * V + j] += g[j] * n;
-          ab[i * V + j] += g[j];
-        }
-      }
-    }
-    if (dx == nullptr) continue;
-    group_sum<G, 2 * R>(s, ws[flip]);
-    flip ^= 1;
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      const uint32_t r = r0 + q * GROUPS + group;
-      if (r >= rows) continue;
-      const float a = layer ? s[2 * q] * inv_c : 0.f, b = s[2 * q + 1] * inv_c;
-#pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-        const int c = (t + i * G) * V;
-        if (c >= C) continue;
-        float g[V], v[V];
-        gp[q][i].get(g);
-        xp[q][i].get(v);
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          v[j] = st[q].y * (g[j] * w[i * V + j] - a - (v[j] - st[q].x) * st[q].y * b);
-        store_v<T, V>(dx + (long long)r * C + c, v);
-      }
-    }
-  }
-  if (part == nullptr) return;
-  join_groups<V, G, GROUPS, UPT, true>(aw, ab, t, group);
-  if (group == 0) store_partial<V, G, UPT, true>(aw, ab, t, C, vec.fp32, part, dw, db);
-}
-
-// ---- staged form: 16-byte fragments through a ring in shared memory
-// Each thread copies its own fragments (dy, x or its codes and scale word) DEPTH - 1 row batches ahead
-// with asynchronous copies and waits for its own copies only, so loads stay in flight across the
-// reductions without holding registers; the second use of a fragment (dx, after the reduction) reads it from the ring again.
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int bytes, bool in) {
-  const int n = in ? bytes : 0;  // 0: the destination is zero-filled, the source is not read
-  if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-  else if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+// ---------------------------------------------------------------- staged form
+// Each thread copies its own fragments DEPTH - 1 row batches ahead with asynchronous copies and waits
+// for its own copies only, so loads stay in flight across the reductions without holding registers and
+// without barriers between copying and using.  Slots of columns past the row's end are zeroed once.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <typename T, int G, int UPT, int R, int DEPTH, bool KEPT>
-struct Staged {
-  static constexpr int NT = G > kThreads ? G : kThreads, GROUPS = NT / G;
-  static constexpr int Q = sizeof(T) / 2;                 // 16-byte pieces of a fragment of T
-  static constexpr int PIECE = NT * 16, SLOTS = R * UPT;  // one piece of every thread; fragments of a stage
-  static constexpr int STAGE = SLOTS * (Q * PIECE + (KEPT ? NT * 12 : Q * PIECE));
-  static constexpr int BYTES = DEPTH * STAGE;
+// One ring of fragments: SLOTS of every thread a stage, Q 16-byte pieces a fragment (bf16 1, fp32 2).
+template <typename T, int NT, int SLOTS>
+struct Ring {
+  static constexpr int Q = sizeof(T) / 2, PIECE = NT * 16, STAGE = SLOTS * Q * PIECE;
+  __device__ __forceinline__ static void fetch(uint32_t stage, int slot, const T* p) {
+#pragma unroll
+    for (int h = 0; h < Q; ++h)
+      copy_async<16>(stage + (slot * Q + h) * PIECE + threadIdx.x * 16, reinterpret_cast<const uint4*>(p) + h);
+  }
+  __device__ __forceinline__ static void get(const uint8_t* stage, int slot, Frag<T>& f) {
+    const uint8_t* at = stage + slot * Q * PIECE + threadIdx.x * 16;
+    if constexpr (Q == 1) {
+      f.raw = *reinterpret_cast<const uint4*>(at);
+    } else {
+      f.raw[0] = *reinterpret_cast<const float4*>(at);
+      f.raw[1] = *reinterpret_cast<const float4*>(at + PIECE);
+    }
+  }
+};
+// The same for codes: 8 bytes a fragment, then the 4-byte word of scales that holds its block's.
+template <int NT, int SLOTS>
+struct CodeRing {
+  static constexpr int STAGE = SLOTS * NT * 12, SCALES = SLOTS * NT * 8;
+  __device__ __forceinline__ static void fetch(uint32_t stage, int slot, const int8_t* codes, const uint8_t* scales, int c) {
+    copy_async<8>(stage + (slot * NT + threadIdx.x) * 8, codes + c);
+    copy_async<4>(stage + SCALES + (slot * NT + threadIdx.x) * 4, scales + c / kKeptBlock / 4 * 4);
+  }
+  // the codes as numbers, and their step
+  __device__ __forceinline__ static float get(const uint8_t* stage, int slot, int c, float2 (&v)[4]) {
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(stage + SCALES + (slot * NT + threadIdx.x) * 4);
+    const uint32_t b = (word >> (c / kKeptBlock % 4 * 8)) & 0xffu;  // 0 in a slot past the row's end, where codes are 0
+    kept8_numbers(*reinterpret_cast<const uint2*>(stage + (slot * NT + threadIdx.x) * 8), v);
+    return kept8_step(b);
+  }
 };
 
+__device__ __forceinline__ void zero_ring(uint8_t* ring, int bytes) {
+  for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16) *reinterpret_cast<uint4*>(ring + i) = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+}
+
+// R rows a group a turn.  x is read once: into the ring, from there into registers, which the mean, the centred squares, the
+// codes and y all use.
+template <typename T, int G, int UPT, int R, int DEPTH, int CTAS, bool LAYER>
+__global__ void __launch_bounds__(threads_of(G), CTAS)
+    norm_fwd_staged_kernel(RowView x, uint32_t rows, int C, Vectors vec, float eps, T* __restrict__ y,
+                           float* __restrict__ stats, Kept k) {
+  constexpr int NT = threads_of(G), GROUPS = NT / G;
+  using X = Ring<T, NT, R * UPT>;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float ws[2][2][NT / 32 * R];
+  const int t = threadIdx.x % G, group = threadIdx.x / G;
+  const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring);
+  const uint64_t step = (uint64_t)gridDim.x * (GROUPS * R);
+  const uint32_t first = blockIdx.x * (GROUPS * R);
+  if (C < G * UPT * 8) zero_ring(ring, DEPTH * X::STAGE);
+
+  auto fetch = [&](uint64_t r0, int stage) {
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const uint64_t r = r0 + q * GROUPS + group;
+      if (r >= rows) continue;
+      const T* p = row_ptr<T>(x, (uint32_t)r);
+#pragma unroll
+      for (int i = 0; i < UPT; ++i)
+        if ((t + i * G) * 8 < C) X::fetch(ring0 + stage * X::STAGE, q * UPT + i, p + (t + i * G) * 8);
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; ++d) {
+    fetch(first + d * step, d);
+    copy_commit();
+  }
+  float2 w[UPT][4], b[LAYER ? UPT : 1][4];
+#pragma unroll
+  for (int i = 0; i < UPT; ++i) {
+    load_pairs(vec.w, vec.fp32, (t + i * G) * 8, C, 1.f, w[i]);
+    if (LAYER) load_pairs(vec.b, vec.fp32, (t + i * G) * 8, C, 0.f, b[i]);
+  }
+  const float inv_c = 1.f / C;
+  int stage = 0, flip = 0;
+  for (uint64_t r0 = first; r0 < rows; r0 += step) {
+    fetch(r0 + (DEPTH - 1) * step, stage == 0 ? DEPTH - 1 : stage - 1);  // into the stage of the last turn
+    copy_commit();
+    copy_wait<DEPTH - 1>();
+    Frag<T> f[R][UPT];
+    float mean[R], var[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      float2 s = twice(0.f);
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        X::get(ring + stage * X::STAGE, q * UPT + i, f[q][i]);
+        if (LAYER) {
+          float2 v[4];
+          f[q][i].get(v);
+          s = add2(s, add2(add2(v[0], v[1]), add2(v[2], v[3])));
+        }
+      }
+      mean[q] = s.x + s.y;
+    }
+    if (LAYER) group_sum<G, R>(mean, ws[flip][0]);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      mean[q] = LAYER ? mean[q] * inv_c : 0.f;
+      float2 s = twice(0.f);
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        if ((t + i * G) * 8 >= C) continue;
+        float2 v[4];
+        f[q][i].get(v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (LAYER) v[j] = add2(v[j], twice(-mean[q]));
+          s = fma2(v[j], v[j], s);
+        }
+      }
+      var[q] = s.x + s.y;
+    }
+    group_sum<G, R>(var, ws[flip][1]);
+    flip ^= 1;
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const uint64_t r = r0 + q * GROUPS + group;
+      const bool in = r < rows;
+      const float rstd = rsqrtf(var[q] * inv_c + eps);
+      if (in && t == 0 && stats != nullptr) *reinterpret_cast<float2*>(stats + 2 * r) = make_float2(mean[q], rstd);
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        const int c = (t + i * G) * 8;
+        if (k.codes != nullptr) {  // all lanes: a block is four of them, zeros past the row's end
+          uint32_t sb;
+          uint2 codes;
+          kept8_encode(f[q][i], sb, codes);
+          if (in && c < k.Cp) {
+            *reinterpret_cast<uint2*>(k.codes + (long long)r * k.Cp + c) = codes;
+            if (c % kKeptBlock == 0) kept8_store_byte(k.scales + (long long)r * k.nbp, c / kKeptBlock, k.nb, k.nbp, sb);
+          }
+        }
+        if (!in || c >= C) continue;
+        float2 v[4];
+        f[q][i].get(v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (LAYER) v[j] = fma2(mul2(add2(v[j], twice(-mean[q])), twice(rstd)), w[i][j], b[LAYER ? i : 0][j]);
+          else v[j] = mul2(mul2(v[j], twice(rstd)), w[i][j]);
+        }
+        store_pairs(y + (long long)r * C + c, v);
+      }
+    }
+    stage = stage == DEPTH - 1 ? 0 : stage + 1;
+  }
+  copy_wait<0>();
+}
+
+// The CTA's groups hold the same columns: add them up, in a fixed order, into the first group.  P values a thread.
+template <int G, int GROUPS, int P>
+__device__ __forceinline__ void join_groups(float (&acc)[P], int t, int group) {
+  if constexpr (GROUPS > 1) {
+    __shared__ float cs[GROUPS / 2 * G * 4];
+#pragma unroll
+    for (int i = 0; i < P; i += 4) {
+#pragma unroll
+      for (int h = GROUPS / 2; h > 0; h >>= 1) {
+        __syncthreads();
+        if (group >= h && group < 2 * h) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) cs[((group - h) * 4 + j) * G + t] = acc[i + j];
+        }
+        __syncthreads();
+        if (group < h) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i + j] += cs[(group * 4 + j) * G + t];
+        }
+      }
+    }
+  }
+}
+
+// Column c of the CTA's partial row; a lone CTA's is the result.
+__device__ __forceinline__ void store_partial(float v, int c, int C, int which, bool fp32, float* part, void* out) {
+  if (gridDim.x > 1) part[((long long)blockIdx.x * 2 + which) * C + c] = v;
+  else if (fp32) store_out<float>(out, c, v);
+  else store_out<__nv_bfloat16>(out, c, v);
+}
+
+// R rows a group a turn; dy and x (or its codes) are read from the ring twice: for the sums and dw / db, then for dx.
 template <typename T, int G, int UPT, int R, int DEPTH, int CTAS, bool LAYER, bool KEPT>
-__global__ void __launch_bounds__(G > kThreads ? G : kThreads, CTAS)
+__global__ void __launch_bounds__(threads_of(G), CTAS)
     norm_bwd_staged_kernel(RowView dy, RowView x, Kept k, uint32_t rows, int C, Vectors vec,
                            const float* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, void* dw,
                            void* db) {
-  using S = Staged<T, G, UPT, R, DEPTH, KEPT>;
-  constexpr int V = 8, NT = S::NT, GROUPS = S::GROUPS, E = UPT * V, N = LAYER ? 2 : 1;
+  constexpr int NT = threads_of(G), GROUPS = NT / G, N = LAYER ? 2 : 1;
+  using D = Ring<T, NT, R * UPT>;
+  using X = Ring<T, NT, R * UPT>;
+  using XK = CodeRing<NT, R * UPT>;
+  constexpr int STAGE = D::STAGE + (KEPT ? XK::STAGE : X::STAGE);
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float ws[2][NT / 32 * N * R];
   const int t = threadIdx.x % G, group = threadIdx.x / G;
   const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring);
-  // byte offsets inside a stage: dy pieces, then x pieces or codes and scale words
-  constexpr int X0 = S::SLOTS * S::Q * S::PIECE, SC0 = X0 + S::SLOTS * NT * 8;
-  const uint32_t step = gridDim.x * (GROUPS * R);
+  const uint64_t step = (uint64_t)gridDim.x * (GROUPS * R);
+  const uint32_t first = blockIdx.x * (GROUPS * R);
+  if (C < G * UPT * 8) zero_ring(ring, DEPTH * STAGE);
 
-  auto fetch = [&](uint32_t r0, int stage) {
+  auto fetch = [&](uint64_t r0, int stage) {
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      const uint32_t r = r0 + q * GROUPS + group;
-      const bool row_in = r >= r0 && r < rows;  // r0 past the rows (or wrapped around): zeros
-      const uint32_t rr = row_in ? r : 0;
-      const T* gr = row_ptr<T>(dy, rr);
+      const uint64_t r = r0 + q * GROUPS + group;
+      if (r >= rows) continue;
+      const uint32_t at = ring0 + stage * STAGE;
+      const T* gr = row_ptr<T>(dy, (uint32_t)r);
+      const T* xr = KEPT ? nullptr : row_ptr<T>(x, (uint32_t)r);
+      const int8_t* codes = KEPT ? k.codes + (long long)r * k.Cp : nullptr;
+      const uint8_t* scales = KEPT ? k.scales + (long long)r * k.nbp : nullptr;
 #pragma unroll
       for (int i = 0; i < UPT; ++i) {
-        const int c = (t + i * G) * V, slot = q * UPT + i;
-        const bool in = row_in && c < C;
-        const int cc = in ? c : 0;
-        const uint32_t at = ring0 + stage * S::STAGE;
-#pragma unroll
-        for (int h = 0; h < S::Q; ++h)
-          copy_async(at + (slot * S::Q + h) * S::PIECE + threadIdx.x * 16, reinterpret_cast<const uint4*>(gr + cc) + h, 16, in);
-        if constexpr (KEPT) {
-          copy_async(at + X0 + (slot * NT + threadIdx.x) * 8, k.codes + (long long)rr * k.Cp + cc, 8, in);
-          copy_async(at + SC0 + (slot * NT + threadIdx.x) * 4,
-                     k.scales + (long long)rr * k.nbp + cc / kKeptBlock / 4 * 4, 4, in);
-        } else {
-          const T* xr = row_ptr<T>(x, rr);
-#pragma unroll
-          for (int h = 0; h < S::Q; ++h)
-            copy_async(at + X0 + (slot * S::Q + h) * S::PIECE + threadIdx.x * 16, reinterpret_cast<const uint4*>(xr + cc) + h, 16, in);
-        }
+        const int c = (t + i * G) * 8, slot = q * UPT + i;
+        if (c >= C) continue;
+        D::fetch(at, slot, gr + c);
+        if constexpr (KEPT) XK::fetch(at + D::STAGE, slot, codes, scales, c);
+        else X::fetch(at + D::STAGE, slot, xr + c);
       }
     }
   };
-  auto dy_of = [&](int stage, int slot, float (&v)[V]) {
-    Pack<T, V> p;
-    const uint8_t* at = ring + stage * S::STAGE + slot * S::Q * S::PIECE + threadIdx.x * 16;
-    if constexpr (sizeof(T) == 2) {
-      p.raw = *reinterpret_cast<const uint4*>(at);
-    } else {
-      p.raw[0] = *reinterpret_cast<const float4*>(at);
-      p.raw[1] = *reinterpret_cast<const float4*>(at + S::PIECE);
-    }
-    p.get(v);
-  };
-  auto x_of = [&](int stage, int slot, int c, float (&v)[V]) {
-    const uint8_t* at = ring + stage * S::STAGE;
+  // dy, and v with (x - mean) = v * unit: a layer norm subtracts the mean here (unit 1), an RMS norm leaves codes as they
+  // are and passes their step on
+  auto get = [&](int stage, int slot, int c, float mean, float2 (&g)[4], float2 (&v)[4]) -> float {
+    const uint8_t* at = ring + stage * STAGE;
+    Frag<T> f;
+    D::get(at, slot, f);
+    f.get(g);
+    float unit = 1.f;
     if constexpr (KEPT) {
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(at + SC0 + (slot * NT + threadIdx.x) * 4);
-      // a zero word (nothing copied) is no scale; its codes are zero
-      const uint32_t b = word == 0 ? kKeptPadByte : (word >> (c / kKeptBlock % 4 * 8)) & 0xffu;
-      kept8_values(*reinterpret_cast<const uint2*>(at + X0 + (slot * NT + threadIdx.x) * 8), kept8_step(b), v);
+      unit = XK::get(at + D::STAGE, slot, c, v);
     } else {
-      Pack<T, V> p;
-      at += X0 + slot * S::Q * S::PIECE + threadIdx.x * 16;
-      if constexpr (sizeof(T) == 2) {
-        p.raw = *reinterpret_cast<const uint4*>(at);
-      } else {
-        p.raw[0] = *reinterpret_cast<const float4*>(at);
-        p.raw[1] = *reinterpret_cast<const float4*>(at + S::PIECE);
-      }
-      p.get(v);
+      X::get(at + D::STAGE, slot, f);
+      f.get(v);
     }
+    if constexpr (LAYER) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = KEPT ? fma2(v[j], twice(unit), twice(-mean)) : add2(v[j], twice(-mean));
+      unit = 1.f;
+    }
+    return unit;
   };
-
-  const uint32_t first = blockIdx.x * (GROUPS * R);
 #pragma unroll
   for (int d = 0; d < DEPTH - 1; ++d) {
-    fetch((uint64_t)first + (uint64_t)d * step < rows ? first + d * step : rows, d);
+    fetch(first + d * step, d);
     copy_commit();
   }
-  float w[E], aw[E], ab[LAYER ? E : 1];
+  float2 w[UPT][4], aw[UPT][4], ab[LAYER ? UPT : 1][4];
 #pragma unroll
   for (int i = 0; i < UPT; ++i) {
-    float v[V];
-    const int c = (t + i * G) * V;
-    load_vec<V>(c < C ? vec.w : nullptr, vec.fp32, c, 1.f, v);
+    load_pairs(vec.w, vec.fp32, (t + i * G) * 8, C, 1.f, w[i]);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      w[i * V + j] = v[j];
-      aw[i * V + j] = 0.f;
-      if (LAYER) ab[i * V + j] = 0.f;
+    for (int j = 0; j < 4; ++j) {
+      aw[i][j] = twice(0.f);
+      if (LAYER) ab[i][j] = twice(0.f);
     }
   }
   const float inv_c = 1.f / C;
   float2 next[R];
-  auto stats_of = [&](uint32_t r0) {
+  auto stats_of = [&](uint64_t r0) {
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      const uint32_t r = r0 + q * GROUPS + group;
-      next[q] = r >= r0 && r < rows ? *reinterpret_cast<const float2*>(stats + 2 * (size_t)r) : make_float2(0.f, 0.f);
+      const uint64_t r = r0 + q * GROUPS + group;
+      next[q] = r < rows ? *reinterpret_cast<const float2*>(stats + 2 * r) : make_float2(0.f, 0.f);
     }
   };
   stats_of(first);
   int stage = 0, flip = 0;
-  for (uint64_t r64 = first; r64 < rows; r64 += step) {
-    const uint32_t r0 = (uint32_t)r64;
+  for (uint64_t r0 = first; r0 < rows; r0 += step) {
     float2 st[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) st[q] = next[q];
-    const int ahead = stage == 0 ? DEPTH - 1 : stage - 1;  // the stage consumed in the last turn
-    const uint64_t r_ahead = r64 + (uint64_t)(DEPTH - 1) * step;
-    fetch(r_ahead < rows ? (uint32_t)r_ahead : rows, ahead);
+    fetch(r0 + (DEPTH - 1) * step, stage == 0 ? DEPTH - 1 : stage - 1);  // into the stage of the last turn
     copy_commit();
-    stats_of(r64 + step < rows ? r0 + step : rows);
+    stats_of(r0 + step);
     copy_wait<DEPTH - 1>();
+    // with d = x - mean and g' = dy w rstd:  s = (sum g' d, sum g'),  dw += dy rstd d,  db += dy
     float s[N * R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
+      float2 sn = twice(0.f), sg = twice(0.f);
+      if (r0 + q * GROUPS + group < rows) {  // a slot without a row holds another row's values
 #pragma unroll
-      for (int n = 0; n < N; ++n) s[q * N + n] = 0.f;
+        for (int i = 0; i < UPT; ++i) {
+          float2 g[4], v[4];
+          const float2 scale = twice(st[q].y * get(stage, q * UPT + i, (t + i * G) * 8, st[q].x, g, v));
 #pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-        float g[V], v[V];
-        dy_of(stage, q * UPT + i, g);
-        x_of(stage, q * UPT + i, (t + i * G) * V, v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float d = LAYER ? v[j] - st[q].x : v[j];
-          const float gw = g[j] * w[i * V + j];
-          s[q * N] += gw * d;
-          aw[i * V + j] += g[j] * (d * st[q].y);
-          if (LAYER) {
-            s[q * N + N - 1] += gw;
-            ab[i * V + j] += g[j];
+          for (int j = 0; j < 4; ++j) {
+            const float2 gr = mul2(g[j], scale);
+            const float2 gw = mul2(gr, w[i][j]);
+            sn = fma2(gw, v[j], sn);
+            aw[i][j] = fma2(gr, v[j], aw[i][j]);
+            if (LAYER) {
+              sg = add2(sg, gw);
+              ab[i][j] = add2(ab[i][j], g[j]);
+            }
           }
         }
       }
+      s[q * N] = sn.x + sn.y;
+      if (LAYER) s[q * N + N - 1] = sg.x + sg.y;
     }
     if (dx != nullptr) {
       group_sum<G, N * R>(s, ws[flip]);
@@ -527,24 +420,25 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads, CTAS)
       asm volatile("" ::: "memory");  // the fragments are read from the ring again, not held in registers
 #pragma unroll
       for (int q = 0; q < R; ++q) {
-        const uint32_t r = r0 + q * GROUPS + group;
+        const uint64_t r = r0 + q * GROUPS + group;
         if (r >= rows) continue;
-        const float rstd = st[q].y;
-        const float a = LAYER ? s[q * N + N - 1] * inv_c * rstd : 0.f;
-        const float b = s[q * N] * inv_c * rstd * rstd * rstd;  // s holds sum gw (x - mean)
+        // dx = g' - mean_c(g') - d rstd^2 mean_c(g' d)
+        const float2 a = twice(LAYER ? -s[q * N + N - 1] * inv_c : 0.f);
+        const float2 b = twice(-s[q * N] * inv_c * st[q].y * st[q].y);
 #pragma unroll
         for (int i = 0; i < UPT; ++i) {
-          const int c = (t + i * G) * V;
+          const int c = (t + i * G) * 8;
           if (c >= C) continue;
-          float g[V], v[V];
-          dy_of(stage, q * UPT + i, g);
-          x_of(stage, q * UPT + i, c, v);
+          float2 g[4], v[4];
+          const float unit = get(stage, q * UPT + i, c, st[q].x, g, v);
+          const float2 bu = LAYER ? b : twice(b.x * unit);
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float d = LAYER ? v[j] - st[q].x : v[j];
-            v[j] = (g[j] * w[i * V + j]) * rstd - a - d * b;
+          for (int j = 0; j < 4; ++j) {
+            float2 gw = mul2(mul2(g[j], twice(st[q].y)), w[i][j]);
+            if (LAYER) gw = add2(gw, a);
+            v[j] = fma2(v[j], bu, gw);
           }
-          store_v<T, V>(dx + (long long)r * C + c, v);
+          store_pairs(dx + (long long)r * C + c, v);
         }
       }
     }
@@ -552,8 +446,173 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads, CTAS)
   }
   copy_wait<0>();
   if (part == nullptr) return;
-  join_groups<V, G, GROUPS, UPT, LAYER>(aw, ab, t, group);
-  if (group == 0) store_partial<V, G, UPT, LAYER>(aw, ab, t, C, vec.fp32, part, dw, db);
+#pragma unroll
+  for (int which = 0; which < N; ++which) {
+#pragma unroll
+    for (int i = 0; i < UPT; ++i) {
+      float acc[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 v = which == 0 ? aw[i][j] : ab[LAYER ? i : 0][j];
+        acc[2 * j] = v.x;
+        acc[2 * j + 1] = v.y;
+      }
+      join_groups<G, GROUPS>(acc, t, group);
+      const int c = (t + i * G) * 8;
+      if (group != 0 || c >= C) continue;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) store_partial(acc[j], c + j, C, which, vec.fp32, part, which == 0 ? dw : db);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- single-column form
+// Rows that 16-byte copies cannot address (odd widths, odd offsets): thread t of a group of whole warps holds columns
+// t + i G, so a warp's 32 neighbouring columns are one block of the codes.
+constexpr int single_ctas(int G) { return threads_of(G) > 512 ? 1 : 768 / threads_of(G); }
+template <typename T, int G, int E, int R>
+__global__ void __launch_bounds__(threads_of(G), single_ctas(G))
+    norm_fwd_single_kernel(RowView x, uint32_t rows, int C, Vectors vec, float eps, bool layer, T* __restrict__ y,
+                           float* __restrict__ stats, Kept k) {
+  constexpr int NT = threads_of(G), GROUPS = NT / G;
+  __shared__ float ws[2][2][NT / 32 * R];
+  const int t = threadIdx.x % G, group = threadIdx.x / G;
+  float w[E], b[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    w[i] = t + i * G < C ? vec_at(vec.w, vec.fp32, t + i * G, 1.f) : 0.f;
+    b[i] = t + i * G < C ? vec_at(vec.b, vec.fp32, t + i * G, 0.f) : 0.f;
+  }
+  const float inv_c = 1.f / C;
+  int flip = 0;
+  for (uint64_t r0 = (uint64_t)blockIdx.x * (GROUPS * R); r0 < rows; r0 += (uint64_t)gridDim.x * (GROUPS * R)) {
+    float v[R][E], mean[R], var[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const uint64_t r = r0 + q * GROUPS + group;
+      const T* xr = row_ptr<T>(x, r < rows ? (uint32_t)r : 0);
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[q][i] = r < rows && t + i * G < C ? to_f32(xr[t + i * G]) : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      mean[q] = var[q] = 0.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) mean[q] += v[q][i];
+    }
+    if (layer) group_sum<G, R>(mean, ws[flip][0]);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      mean[q] = layer ? mean[q] * inv_c : 0.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const float d = t + i * G < C ? v[q][i] - mean[q] : 0.f;
+        var[q] += d * d;
+      }
+    }
+    group_sum<G, R>(var, ws[flip][1]);
+    flip ^= 1;
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const uint64_t r = r0 + q * GROUPS + group;
+      const bool in = r < rows;
+      const float rstd = rsqrtf(var[q] * inv_c + eps);
+      if (in && t == 0 && stats != nullptr) *reinterpret_cast<float2*>(stats + 2 * r) = make_float2(mean[q], rstd);
+      T* yr = y + (long long)r * C;
+      int8_t* codes = k.codes + (long long)r * k.Cp;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int c = t + i * G;
+        if (k.codes != nullptr && c - (int)(threadIdx.x & 31) < C) {  // whole warps: blocks that the row reaches
+          const float one[1] = {v[q][i]};
+          const uint32_t sb = kept8_byte(kept8_amax<1>(one));
+          if (in) {
+            kept8_store_codes<1>(codes + c, one, sb);
+            if (c % kKeptBlock == 0) kept8_store_byte(k.scales + (long long)r * k.nbp, c / kKeptBlock, k.nb, k.nbp, sb);
+          }
+        }
+        if (in && c < C) yr[c] = from_f32<T>((v[q][i] - mean[q]) * rstd * w[i] + b[i]);
+      }
+    }
+  }
+}
+
+template <typename T, int G, int E, int R, bool KEPT>
+__global__ void __launch_bounds__(threads_of(G), 512 / threads_of(G) > 0 ? 512 / threads_of(G) : 1)
+    norm_bwd_single_kernel(RowView dy, RowView x, Kept k, uint32_t rows, int C, Vectors vec, bool layer,
+                           const float* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, void* dw,
+                           void* db) {
+  constexpr int NT = threads_of(G), GROUPS = NT / G;
+  __shared__ float ws[2][NT / 32 * 2 * R];
+  const int t = threadIdx.x % G, group = threadIdx.x / G, lane = threadIdx.x & 31;
+  float w[E], aw[E], ab[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    w[i] = t + i * G < C ? vec_at(vec.w, vec.fp32, t + i * G, 1.f) : 0.f;
+    aw[i] = ab[i] = 0.f;
+  }
+  const float inv_c = 1.f / C;
+  int flip = 0;
+  for (uint64_t r0 = (uint64_t)blockIdx.x * (GROUPS * R); r0 < rows; r0 += (uint64_t)gridDim.x * (GROUPS * R)) {
+    float g[R][E], v[R][E], s[2 * R], step[R];
+    float2 st[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const uint64_t r = r0 + q * GROUPS + group;
+      const bool in = r < rows;
+      const uint32_t rr = in ? (uint32_t)r : 0;
+      const T* gr = row_ptr<T>(dy, rr);
+      const T* xr = KEPT ? nullptr : row_ptr<T>(x, rr);
+      const int8_t* codes = KEPT ? k.codes + (long long)rr * k.Cp : nullptr;
+      st[q] = in ? *reinterpret_cast<const float2*>(stats + 2 * (size_t)rr) : make_float2(0.f, 0.f);
+      if (KEPT) {  // lane i reads the scale of the warp's i-th block of this row
+        const int blk = (t - lane + lane * G) / kKeptBlock;
+        step[q] = in && lane < E && blk < k.nb ? kept8_step(k.scales[(long long)rr * k.nbp + blk]) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const bool at = in && t + i * G < C;
+        g[q][i] = at ? to_f32(gr[t + i * G]) : 0.f;
+        v[q][i] = !at ? 0.f : KEPT ? kept8_number(codes[t + i * G]) : to_f32(xr[t + i * G]);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      s[2 * q] = s[2 * q + 1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if (KEPT) v[q][i] *= __shfl_sync(0xffffffffu, step[q], i);
+        v[q][i] = (v[q][i] - st[q].x) * st[q].y;  // n; columns past the row have g = 0
+        const float gw = g[q][i] * w[i];
+        s[2 * q] += gw;
+        s[2 * q + 1] += t + i * G < C ? gw * v[q][i] : 0.f;
+        aw[i] += g[q][i] * v[q][i];
+        ab[i] += g[q][i];
+      }
+    }
+    if (dx == nullptr) continue;
+    group_sum<G, 2 * R>(s, ws[flip]);
+    flip ^= 1;
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const uint64_t r = r0 + q * GROUPS + group;
+      if (r >= rows) continue;
+      const float a = layer ? s[2 * q] * inv_c : 0.f, b = s[2 * q + 1] * inv_c;
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (t + i * G < C) dx[(long long)r * C + t + i * G] = from_f32<T>(st[q].y * (g[q][i] * w[i] - a - v[q][i] * b));
+    }
+  }
+  if (part == nullptr) return;
+  join_groups<G, GROUPS>(aw, t, group);
+  join_groups<G, GROUPS>(ab, t, group);
+  if (group != 0) return;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    if (t + i * G >= C) continue;
+    store_partial(aw[i], t + i * G, C, 0, vec.fp32, part, dw);
+    store_partial(ab[i], t + i * G, C, 1, vec.fp32, part, db);
+  }
 }
 
 // dw[c], db[c] from the partial rows: 32 columns a CTA, 8 interleaved chains a column, joined in order.
@@ -588,12 +647,6 @@ __device__ __forceinline__ float cta_sum(float v) {
   return s[0];
 }
 
-__device__ __forceinline__ float vec_at(const void* p, bool fp32, int c, float missing) {
-  float v[1];
-  load_vec<1>(p, fp32, c, missing, v);
-  return v[0];
-}
-
 // One CTA per row, three sweeps over it (mean, variance, output).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) norm_fwd_wide_kernel(RowView x, uint32_t rows, int C, Vectors vec,
@@ -612,7 +665,7 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_wide_kernel(RowView x, uint
       var += d * d;
     }
     const float rstd = rsqrtf(cta_sum(var) / C + eps);
-    if (threadIdx.x == 0) *reinterpret_cast<float2*>(stats + 2 * (size_t)r) = make_float2(mean, rstd);
+    if (threadIdx.x == 0 && stats != nullptr) *reinterpret_cast<float2*>(stats + 2 * (size_t)r) = make_float2(mean, rstd);
     T* yr = y + (long long)r * C;
     for (int c = threadIdx.x; c < (k.codes != nullptr ? k.Cp : C); c += kThreads) {
       float v[1] = {c < C ? to_f32(xr[c]) : 0.f};
@@ -708,42 +761,75 @@ int sm_count() {
   return n;
 }
 
+// CTAs for `rows` in batches of `batch`, at most `ctas` on every SM.
+int grid_for(long long rows, int batch, int ctas) {
+  const long long want = (rows + batch - 1) / batch, most = (long long)sm_count() * ctas;
+  return (int)(want < 1 ? 1 : want < most ? want : most);
+}
+
 uint32_t wide_grid(long long rows) { return (uint32_t)(rows < 148 * 64 ? rows : 148 * 64); }
 
-template <typename T, int V, int G, int UPT>
-void fwd_rows(const NormArgs& a, const RowsArg& x, void* y, float* stats, const Kept8Buf& k, cudaStream_t s) {
-  constexpr int NT = G > kThreads ? G : kThreads, GROUPS = NT / G;
-  norm_fwd_kernel<T, V, G, UPT><<<(uint32_t)((a.rows + GROUPS - 1) / GROUPS), NT, 0, s>>>(
-      view_of(x), a.rows, a.C, Vectors{a.w, a.b, a.w_fp32}, a.eps, a.layer, (T*)y, stats, kept_of(k));
+constexpr int kRingBudget = 220 * 1024;  // rings of all resident CTAs of an SM
+
+struct FwdCall {
+  const NormArgs& a;
+  const RowsArg& x;
+  void* y;
+  float* stats;
+  const Kept8Buf& k;
+  cudaStream_t s;
+  Vectors vec() const { return Vectors{a.w, a.b, a.w_fp32}; }
+};
+
+template <typename T, int G, int UPT, int R, int DEPTH, int CTAS, bool LAYER>
+void fwd_staged(const FwdCall& f) {
+  constexpr int NT = threads_of(G), GROUPS = NT / G, BYTES = DEPTH * Ring<T, NT, R * UPT>::STAGE;
+  static_assert(BYTES * CTAS <= kRingBudget, "the rings of an SM's CTAs do not fit its shared memory");
+  const auto kernel = norm_fwd_staged_kernel<T, G, UPT, R, DEPTH, CTAS, LAYER>;
+  static bool ready = false;
+  if (!ready) ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) == cudaSuccess;
+  kernel<<<grid_for(f.a.rows, GROUPS * R, CTAS), NT, BYTES, f.s>>>(view_of(f.x), (uint32_t)f.a.rows, f.a.C, f.vec(),
+                                                                   f.a.eps, (T*)f.y, f.stats, kept_of(f.k));
+}
+
+template <typename T, int G, int E, int R>
+void fwd_single(const FwdCall& f) {
+  constexpr int NT = threads_of(G), GROUPS = NT / G;
+  norm_fwd_single_kernel<T, G, E, R><<<grid_for(f.a.rows, GROUPS * R, single_ctas(G)), NT, 0, f.s>>>(
+      view_of(f.x), (uint32_t)f.a.rows, f.a.C, f.vec(), f.a.eps, f.a.layer, (T*)f.y, f.stats, kept_of(f.k));
+}
+
+template <typename T, bool LAYER>
+void fwd_staged_any(const FwdCall& f) {
+  const int C = f.a.C;
+  constexpr int R = sizeof(T) == 2 ? 2 : 1, CTAS = sizeof(T) == 2 && LAYER ? 2 : 3, DEPTH = CTAS == 2 ? 6 : 4;
+#define STAGED(G) return fwd_staged<T, G, 2, R, DEPTH, CTAS, LAYER>(f)
+  if (C <= 64) STAGED(4);
+  if (C <= 128) STAGED(8);
+  if (C <= 256) STAGED(16);
+  if (C <= 512) STAGED(32);
+  if (C <= 1024) STAGED(64);
+  if (C <= 2048) STAGED(128);
+  if (C <= 4096) STAGED(256);
+#undef STAGED
+  if (C <= 8192) return fwd_staged<T, 512, 2, R, 4, 1, LAYER>(f);
+  fwd_staged<T, 512, 4, 1, sizeof(T) == 2 ? 4 : 3, 1, LAYER>(f);
 }
 
 template <typename T>
-void fwd(const NormArgs& a, const RowsArg& x, void* y, float* stats, const Kept8Buf& k, cudaStream_t s) {
-  const int C = a.C;
-#define ROWS(V, G, UPT) return fwd_rows<T, V, G, UPT>(a, x, y, stats, k, s)
-  if (C % 8 == 0 && rows_aligned16(x, a.fp32) && aligned16(a.w) && aligned16(a.b)) {
-    // the smallest group whose threads hold the row in at most 4 fragments up to a warp; then up to
-    // 16 bf16 / 8 fp32 fragments (64 registers), then more warps
-    if (C <= 128) ROWS(8, 4, 4);
-    if (C <= 256) ROWS(8, 8, 4);
-    if (C <= 512) ROWS(8, 16, 4);
-    if (C <= 1024) ROWS(8, 32, 4);
-    if (C <= 2048) ROWS(8, 32, 8);
-    if constexpr (sizeof(T) == 2) {
-      if (C <= 4096) ROWS(8, 32, 16);
-    }
-    if (C <= 8192) ROWS(8, 128, 8);
-    if (C <= 16384) ROWS(8, 256, 8);
-    if (C <= 32768) ROWS(8, 512, 8);
-  } else {
-    if (C <= 256) ROWS(1, 32, 8);
-    if (C <= 1024) ROWS(1, 32, 32);
-    if (C <= 4096) ROWS(1, 128, 32);
-    if (C <= 16384) ROWS(1, 512, 32);
-  }
-#undef ROWS
-  norm_fwd_wide_kernel<T><<<wide_grid(a.rows), kThreads, 0, s>>>(
-      view_of(x), a.rows, C, Vectors{a.w, a.b, a.w_fp32}, a.eps, a.layer, (T*)y, stats, kept_of(k));
+void fwd(const FwdCall& f) {
+  const int C = f.a.C;
+  if (C % 8 == 0 && C <= 16384 && rows_aligned16(f.x, f.a.fp32) && aligned16(f.a.w) && aligned16(f.a.b))
+    return f.a.layer ? fwd_staged_any<T, true>(f) : fwd_staged_any<T, false>(f);
+  if (C <= 256) return fwd_single<T, 32, 8, 4>(f);
+  if (C <= 1024) return fwd_single<T, 128, 8, 4>(f);
+  if (C <= 2048) return fwd_single<T, 256, 8, 4>(f);
+  if (C <= 4096) return fwd_single<T, 256, 16, 2>(f);
+  if (C <= 8192) return fwd_single<T, 512, 16, 2>(f);
+  if (C <= 16384) return fwd_single<T, 1024, 16, 1>(f);
+  norm_fwd_wide_kernel<T><<<wide_grid(f.a.rows), kThreads, 0, f.s>>>(view_of(f.x), (uint32_t)f.a.rows, C, f.vec(),
+                                                                     f.a.eps, f.a.layer, (T*)f.y, f.stats,
+                                                                     kept_of(f.k));
 }
 
 struct BwdCall {
@@ -755,76 +841,66 @@ struct BwdCall {
   float* part;
   void *dw, *db;
   cudaStream_t s;
-  int* parts;  // asked for the number of partial rows instead of a launch when not null
+  int* parts;  // when not null: only the number of partial rows is wanted
+  Vectors vec() const { return Vectors{a.w, nullptr, a.w_fp32}; }
+  void finish(int grid) const {
+    if (part != nullptr && grid > 1)
+      norm_bwd_final_kernel<<<dim3((a.C + 31) / 32, 2), 32 * kFinalChains, 0, s>>>(part, grid, a.C, a.w_fp32, dw, db);
+  }
 };
-
-template <typename T, int V, int G, int UPT, int R, bool KEPT>
-void bwd_rows(const BwdCall& b) {
-  constexpr int NT = G > kThreads ? G : kThreads, GROUPS = NT / G;
-  static int resident = 0;
-  if (resident == 0) {
-    int n = 0;
-    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, norm_bwd_kernel<T, V, G, UPT, R, KEPT>, NT, 0);
-    resident = n < 1 ? 1 : n;
-  }
-  const long long want = (b.a.rows + GROUPS * R - 1) / (GROUPS * R), most = (long long)sm_count() * resident;
-  const int grid = (int)(want < 1 ? 1 : want < most ? want : most);
-  if (b.parts != nullptr) {
-    *b.parts = grid;
-    return;
-  }
-  norm_bwd_kernel<T, V, G, UPT, R, KEPT><<<grid, NT, 0, b.s>>>(
-      view_of(b.dy), view_of(b.x), kept_of(b.k), b.a.rows, b.a.C, Vectors{b.a.w, nullptr, b.a.w_fp32}, b.a.layer,
-      b.stats, (T*)b.dx, b.part, b.dw, b.db);
-  if (b.part != nullptr && grid > 1)
-    norm_bwd_final_kernel<<<dim3((b.a.C + 31) / 32, 2), 32 * kFinalChains, 0, b.s>>>(b.part, grid, b.a.C, b.a.w_fp32,
-                                                                                     b.dw, b.db);
-}
 
 template <typename T, int G, int UPT, int R, int DEPTH, int CTAS, bool LAYER, bool KEPT>
 void bwd_staged(const BwdCall& b) {
-  using S = Staged<T, G, UPT, R, DEPTH, KEPT>;
-  static_assert(S::BYTES * CTAS <= 220 * 1024, "the rings of an SM's CTAs do not fit its shared memory");
-  const auto kernel = norm_bwd_staged_kernel<T, G, UPT, R, DEPTH, CTAS, LAYER, KEPT>;
-  static bool ready = false;
-  if (!ready) {
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
-    ready = true;
-  }
-  const long long want = (b.a.rows + S::GROUPS * R - 1) / (S::GROUPS * R), most = (long long)sm_count() * CTAS;
-  const int grid = (int)(want < 1 ? 1 : want < most ? want : most);
+  constexpr int NT = threads_of(G), GROUPS = NT / G;
+  using D = Ring<T, NT, R * UPT>;
+  constexpr int BYTES = DEPTH * (D::STAGE + (KEPT ? CodeRing<NT, R * UPT>::STAGE : D::STAGE));
+  static_assert(BYTES * CTAS <= kRingBudget, "the rings of an SM's CTAs do not fit its shared memory");
+  const int grid = grid_for(b.a.rows, GROUPS * R, CTAS);
   if (b.parts != nullptr) {
     *b.parts = grid;
     return;
   }
-  kernel<<<grid, S::NT, S::BYTES, b.s>>>(view_of(b.dy), view_of(b.x), kept_of(b.k), b.a.rows, b.a.C,
-                                         Vectors{b.a.w, nullptr, b.a.w_fp32}, b.stats, (T*)b.dx, b.part, b.dw, b.db);
-  if (b.part != nullptr && grid > 1)
-    norm_bwd_final_kernel<<<dim3((b.a.C + 31) / 32, 2), 32 * kFinalChains, 0, b.s>>>(b.part, grid, b.a.C, b.a.w_fp32,
-                                                                                     b.dw, b.db);
+  const auto kernel = norm_bwd_staged_kernel<T, G, UPT, R, DEPTH, CTAS, LAYER, KEPT>;
+  static bool ready = false;
+  if (!ready) ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) == cudaSuccess;
+  kernel<<<grid, NT, BYTES, b.s>>>(view_of(b.dy), view_of(b.x), kept_of(b.k), (uint32_t)b.a.rows, b.a.C, b.vec(),
+                                   b.stats, (T*)b.dx, b.part, b.dw, b.db);
+  b.finish(grid);
 }
 
-template <typename T, bool KEPT>
+template <typename T, int G, int E, int R, bool KEPT>
+void bwd_single(const BwdCall& b) {
+  constexpr int NT = threads_of(G), GROUPS = NT / G;
+  const int grid = grid_for(b.a.rows, GROUPS * R, 512 / NT > 0 ? 512 / NT : 1);
+  if (b.parts != nullptr) {
+    *b.parts = grid;
+    return;
+  }
+  norm_bwd_single_kernel<T, G, E, R, KEPT><<<grid, NT, 0, b.s>>>(view_of(b.dy), view_of(b.x), kept_of(b.k),
+                                                                 (uint32_t)b.a.rows, b.a.C, b.vec(), b.a.layer,
+                                                                 b.stats, (T*)b.dx, b.part, b.dw, b.db);
+  b.finish(grid);
+}
+
+template <typename T>
 void bwd_wide(const BwdCall& b) {
   const NormArgs& a = b.a;
-  const int parts = (int)(a.rows < 128 ? 1 : a.rows > 1024 * 128 ? 1024 : (a.rows + 127) / 128);
+  const int parts = (int)(a.rows < 128 ? 2 : a.rows > 1024 * 128 ? 1024 : (a.rows + 127) / 128 + 1);
   if (b.parts != nullptr) {
     *b.parts = parts;
     return;
   }
-  const Vectors vec{a.w, nullptr, a.w_fp32};
   if (b.dx != nullptr && a.rows > 0)
-    norm_bwd_wide_dx_kernel<T><<<wide_grid(a.rows), kThreads, 0, b.s>>>(view_of(b.dy), view_of(b.x), kept_of(b.k),
-                                                                        a.rows, a.C, vec, a.layer, b.stats, (T*)b.dx);
+    norm_bwd_wide_dx_kernel<T><<<wide_grid(a.rows), kThreads, 0, b.s>>>(
+        view_of(b.dy), view_of(b.x), kept_of(b.k), (uint32_t)a.rows, a.C, b.vec(), a.layer, b.stats, (T*)b.dx);
   if (b.part == nullptr) return;
   norm_bwd_wide_partial_kernel<T><<<dim3((a.C + kThreads - 1) / kThreads, parts), kThreads, 0, b.s>>>(
-      view_of(b.dy), view_of(b.x), kept_of(b.k), a.rows, a.C, b.stats, (uint32_t)((a.rows + parts - 1) / parts),
-      b.part);
-  norm_bwd_final_kernel<<<dim3((a.C + 31) / 32, 2), 32 * kFinalChains, 0, b.s>>>(b.part, parts, a.C, a.w_fp32, b.dw,
-                                                                                 b.db);
+      view_of(b.dy), view_of(b.x), kept_of(b.k), (uint32_t)a.rows, a.C, b.stats,
+      (uint32_t)((a.rows + parts - 1) / parts), b.part);
+  b.finish(parts);
 }
 
-// 16 columns a thread, so 16 accumulators for each of dw and db; 2 CTAs an SM with rings of about 100 KB
+// 16 columns a thread, so 16 accumulators for each of dw and db
 template <typename T, bool LAYER, bool KEPT>
 void bwd_staged_any(const BwdCall& b) {
   const int C = b.a.C;
@@ -839,7 +915,7 @@ void bwd_staged_any(const BwdCall& b) {
   if (C <= 4096) STAGED(256);
 #undef STAGED
   if (C <= 8192) return bwd_staged<T, 512, 2, R, 3, 1, LAYER, KEPT>(b);
-  bwd_staged<T, 512, 4, 1, 6 / (int)sizeof(T), 1, LAYER, KEPT>(b);
+  bwd_staged<T, 512, 4, 1, sizeof(T) == 2 ? 3 : KEPT ? 2 : 1, 1, LAYER, KEPT>(b);
 }
 
 template <typename T, bool KEPT>
@@ -848,14 +924,12 @@ void bwd(const BwdCall& b) {
   const bool fp32 = sizeof(T) == 4;
   if (C % 8 == 0 && C <= 16384 && rows_aligned16(b.dy, fp32) && (KEPT || rows_aligned16(b.x, fp32)) && aligned16(b.a.w))
     return b.a.layer ? bwd_staged_any<T, true, KEPT>(b) : bwd_staged_any<T, false, KEPT>(b);
-#define ROWS(G, UPT, R) return bwd_rows<T, 1, G, UPT, R, KEPT>(b)
-  if (C <= 256) ROWS(32, 8, 4);
-  if (C <= 512) ROWS(32, 16, 2);
-  if (C <= 2048) ROWS(128, 16, 2);
-  if (C <= 4096) ROWS(256, 16, 2);
-  if (C <= 8192) ROWS(512, 16, 1);
-#undef ROWS
-  bwd_wide<T, KEPT>(b);
+  if (C <= 256) return bwd_single<T, 32, 8, 2, KEPT>(b);
+  if (C <= 1024) return bwd_single<T, 128, 8, 2, KEPT>(b);
+  if (C <= 2048) return bwd_single<T, 256, 8, 2, KEPT>(b);
+  if (C <= 4096) return bwd_single<T, 512, 8, 1, KEPT>(b);
+  if (C <= 8192) return bwd_single<T, 1024, 8, 1, KEPT>(b);
+  bwd_wide<T>(b);
 }
 
 void bwd_any(const BwdCall& b) {
@@ -867,7 +941,8 @@ void bwd_any(const BwdCall& b) {
 
 void launch_norm_fwd(const NormArgs& a, const RowsArg& x, void* y, float* stats, const Kept8Buf& k, cudaStream_t s) {
   if (a.rows <= 0) return;
-  a.fp32 ? fwd<float>(a, x, y, stats, k, s) : fwd<__nv_bfloat16>(a, x, y, stats, k, s);
+  const FwdCall f{a, x, y, stats, k, s};
+  a.fp32 ? fwd<float>(f) : fwd<__nv_bfloat16>(f);
 }
 
 int norm_bwd_parts(const NormArgs& a, const RowsArg& dy, const RowsArg& x, const Kept8Buf& k) {

@@ -32,8 +32,6 @@ from ._ext import ext
 from .gemm import _pad_k, mm_nn, mm_nt, mm_tn
 
 BLOCK = 32
-# rows of the kept input reloaded at a time for a weight gradient (bounds the bf16 temporary)
-WGRAD_ROW_CHUNK = 16384
 
 
 class Kept8:
@@ -110,10 +108,7 @@ def _values_cpu(codes: torch.Tensor, scales: torch.Tensor, C: int, dtype: torch.
 
 def keep_codes(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(codes, scales)`` of the rows of ``x``."""
-    if x.is_cuda:
-        codes, scales = ext().keep8(x.detach())
-        return codes, scales
-    return _keep_cpu(x)
+    return ext().keep8(x) if x.is_cuda else _keep_cpu(x)
 
 
 def restore_codes(codes: torch.Tensor, scales: torch.Tensor, C: int, dtype: torch.dtype,
@@ -131,14 +126,12 @@ def restore_codes(codes: torch.Tensor, scales: torch.Tensor, C: int, dtype: torc
 # store and reload
 # --------------------------------------------------------------------------------------------
 
-@torch.no_grad()
 def keep8(x: torch.Tensor) -> Kept8:
     """``x`` (any leading dims and strides) held in 8 bits.  Not differentiable."""
     check_activation(x, "x")
     return Kept8(*keep_codes(x), x.shape, x.dtype)
 
 
-@torch.no_grad()
 def restore8(kept: Kept8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """The values of ``kept`` as a contiguous tensor of its shape, in its dtype (or ``dtype``)."""
     if not isinstance(kept, Kept8):
@@ -175,28 +168,13 @@ def _bias_operand(b: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return torch.nn.functional.pad(b, (0, _pad8(b.shape[0]) - b.shape[0])).contiguous()
 
 
-def weight_grads8(grads, codes: torch.Tensor, scales: torch.Tensor, K: int, dtypes):
-    """``[g^T x for g in grads]`` with ``x [rows, K]`` the kept matrix: the weight gradients of the
-    projections that read it.  ``grads`` are ``[rows, N]``, ``dtypes`` the result types."""
-    rows = codes.shape[0]
-    if not codes.is_cuda:
-        x = _values_cpu(codes, scales, K, wide_dtype(grads[0].dtype))
-        return [(g.to(x.dtype).t() @ x).to(dt) for g, dt in zip(grads, dtypes)]
-    if rows == 0:
-        return [torch.zeros(g.shape[1], K, dtype=dt, device=codes.device) for g, dt in zip(grads, dtypes)]
-    one = rows <= WGRAD_ROW_CHUNK
-    outs = []
-    for r0 in range(0, rows, WGRAD_ROW_CHUNK):
-        n = min(WGRAD_ROW_CHUNK, rows - r0)
-        x = torch.empty(n, _pad8(K), dtype=torch.bfloat16, device=codes.device)
-        ext().restore8(codes, scales, K, r0, x)  # padding columns only reach padding columns of the result
-        for i, (g, dt) in enumerate(zip(grads, dtypes)):
-            gp = _pad_k(g[r0:r0 + n], _pad8(g.shape[1]))
-            if r0 == 0:
-                outs.append(mm_tn(gp, x, out_dtype=torch.bfloat16 if one and dt == torch.bfloat16 else torch.float32))
-            else:
-                mm_tn(gp, x, out=outs[i], accumulate=True)
-    return [o[:g.shape[1], :K].to(dt) for o, g, dt in zip(outs, grads, dtypes)]
+def weight_grad8(g: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, K: int, dtype) -> torch.Tensor:
+    """``g^T x`` in ``dtype``, ``x [rows, K]`` the kept matrix and ``g [rows, N]``: the weight gradient of a
+    projection that read ``x``."""
+    if codes.is_cuda:
+        return ext().linear8_weight_grad(g, codes, scales, K, dtype != torch.bfloat16).to(dtype)
+    x = _values_cpu(codes, scales, K, wide_dtype(g.dtype))
+    return (g.to(x.dtype).t() @ x).to(dtype)
 
 
 def row_sum(g: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
@@ -246,13 +224,12 @@ def _check_linear(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor]) -
             raise ValueError(f"{name} is on {t.device}, the input on {x.device}")
 
 
-class _Kept8Linear(torch.autograd.Function):
+class _Kept8LinearCPU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b):
-        K = x.shape[-1]
-        x2 = x.reshape(-1, K)
+        x2 = x.reshape(-1, x.shape[-1])
         y = _project(x2, w, b)
-        codes, scales = keep_codes(x2) if ctx.needs_input_grad[1] else (None, None)
+        codes, scales = _keep_cpu(x2) if ctx.needs_input_grad[1] else (None, None)
         ctx.save_for_backward(codes, scales, w)
         ctx.shape, ctx.b_dtype = x.shape, None if b is None else b.dtype
         return y.reshape(*x.shape[:-1], w.shape[0])
@@ -262,7 +239,7 @@ class _Kept8Linear(torch.autograd.Function):
         codes, scales, w = ctx.saved_tensors
         g2 = gy.reshape(-1, gy.shape[-1])
         gx = _input_grad(g2, w).reshape(ctx.shape) if ctx.needs_input_grad[0] else None
-        gw = weight_grads8([g2], codes, scales, w.shape[1], [w.dtype])[0] if ctx.needs_input_grad[1] else None
+        gw = weight_grad8(g2, codes, scales, w.shape[1], w.dtype) if ctx.needs_input_grad[1] else None
         gb = row_sum(g2, ctx.b_dtype) if ctx.b_dtype is not None and ctx.needs_input_grad[2] else None
         return gx, gw, gb
 
@@ -274,8 +251,8 @@ def kept8_linear(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = N
     widths work (those that are not multiples of 8 are padded)."""
     _check_linear(x, w, b)
     if x.is_cuda:
-        x = x.to(torch.bfloat16)
-    return _Kept8Linear.apply(x, w, b)
+        return ext().linear8(x, w, b)
+    return _Kept8LinearCPU.apply(x, w, b)
 
 
 # --------------------------------------------------------------------------------------------
@@ -285,7 +262,7 @@ def kept8_linear(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = N
 def _swiglu_forward(gate, value):
     """``(h, codes and scales of gate, of value)``."""
     if gate.is_cuda:
-        return ext().swiglu8_fwd(gate, value)
+        return ext().swiglu8_fwd(gate, value, True)
     wide = wide_dtype(gate.dtype)
     g = gate.to(wide)
     h = (g * torch.sigmoid(g) * value.to(wide)).to(gate.dtype)
@@ -304,7 +281,7 @@ def _swiglu_backward(dh, kept, want_h: bool):
     return [t.to(dh.dtype) for t in out]
 
 
-class _Kept8SwiGLU(torch.autograd.Function):
+class _Kept8SwiGLUCPU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, value):
         h, *kept = _swiglu_forward(gate, value)
@@ -322,7 +299,9 @@ def kept8_swiglu(gate: torch.Tensor, value: torch.Tensor) -> torch.Tensor:
     check_activation(gate, "gate")
     check_activation(value, "value")
     _check_match(gate, value, "gate and value")
-    return _Kept8SwiGLU.apply(gate, value)
+    if gate.is_cuda:
+        return ext().swiglu8(gate, value)
+    return _Kept8SwiGLUCPU.apply(gate, value)
 
 
 class _Kept8SwiGLUFFN(torch.autograd.Function):
@@ -346,11 +325,10 @@ class _Kept8SwiGLUFFN(torch.autograd.Function):
             gw2 = _dense_weight_grad(g2, h[0], w2.dtype)
         if need_x:
             gx = _input_grad(dvalue, w3, out=_input_grad(dgate, w1)).reshape(ctx.shape)
-        wanted = [(d, w.dtype) for d, w, need in ((dgate, w1, need_1), (dvalue, w3, need_3)) if need]
-        if wanted:
-            got = weight_grads8([d for d, _ in wanted], codes, scales, w1.shape[1], [t for _, t in wanted])
-            gw1 = got.pop(0) if need_1 else None
-            gw3 = got.pop(0) if need_3 else None
+        if need_1:
+            gw1 = weight_grad8(dgate, codes, scales, w1.shape[1], w1.dtype)
+        if need_3:
+            gw3 = weight_grad8(dvalue, codes, scales, w3.shape[1], w3.dtype)
         return gx, gw1, gw3, gw2
 
 

@@ -21,16 +21,12 @@ from ._ext import ext
 from .kept8 import _keep_cpu, _values_cpu, check_activation, wide_dtype
 
 
-class _Norm(torch.autograd.Function):
+class _NormCPU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, eps, layer, kept8):
-        keep = kept8 and any(ctx.needs_input_grad[:2])
-        if x.is_cuda:
-            y, stats, codes, scales = ext().norm_fwd(x, w, b, eps, layer, keep)
-        else:
-            y, stats = _forward_cpu(x, w, b, eps, layer)
-            codes, scales = _keep_cpu(x) if keep else (None, None)
-        ctx.save_for_backward(None if keep else x, codes, scales, stats, w)
+        y, stats = _forward_cpu(x, w, b, eps, layer)
+        codes, scales = _keep_cpu(x) if kept8 else (None, None)
+        ctx.save_for_backward(None if kept8 else x, codes, scales, stats, w)
         ctx.layer = layer
         ctx.w_dtype = w.dtype if w is not None else b.dtype if b is not None else x.dtype
         return y
@@ -38,13 +34,8 @@ class _Norm(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         x, codes, scales, stats, w = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        if dy.is_cuda:
-            dx, dw, db = ext().norm_bwd(dy, x, codes, scales, stats, w, ctx.layer, need_x, need_w, need_b,
-                                        ctx.w_dtype == torch.float32)
-        else:
-            dx, dw, db = _backward_cpu(dy, x, codes, scales, stats, w, ctx.layer, ctx.w_dtype)
-        return dx if need_x else None, dw if need_w else None, db if need_b else None, None, None, None
+        grads = _backward_cpu(dy, x, codes, scales, stats, w, ctx.layer, ctx.w_dtype)
+        return *(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None
 
 
 def _forward_cpu(x, w, b, eps, layer):
@@ -90,6 +81,14 @@ def _check(x, w, b, eps):
         raise ValueError(f"eps={eps} is negative")
 
 
+def _norm(x, w, b, eps, layer, kept8):
+    _check(x, w, b, eps)
+    w, b = _flat(w), _flat(b)
+    if x.is_cuda:
+        return ext().norm(x, w, b, float(eps), layer, bool(kept8))
+    return _NormCPU.apply(x, w, b, float(eps), layer, bool(kept8))
+
+
 def _flat(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t if t is None or t.is_contiguous() else t.contiguous()
 
@@ -97,12 +96,10 @@ def _flat(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-6, kept8: bool = False) -> torch.Tensor:
     """``(x - mean) * rsqrt(var + eps) * weight + bias`` over the last dim (biased variance)."""
-    _check(x, weight, bias, eps)
-    return _Norm.apply(x, _flat(weight), _flat(bias), float(eps), True, bool(kept8))
+    return _norm(x, weight, bias, eps, True, kept8)
 
 
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
              kept8: bool = False) -> torch.Tensor:
     """``x * rsqrt(mean(x^2) + eps) * weight`` over the last dim."""
-    _check(x, weight, None, eps)
-    return _Norm.apply(x, _flat(weight), None, float(eps), False, bool(kept8))
+    return _norm(x, weight, None, eps, False, kept8)

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import kept8_ref as R
-from pan2_b200.ops.kept8 import (keep8, kept8_linear, kept8_swiglu, kept8_swiglu_ffn, restore8, weight_grads8)
+from pan2_b200.ops.kept8 import (keep8, kept8_linear, kept8_swiglu, kept8_swiglu_ffn, restore8, weight_grad8)
 from pan2_b200.ops.norm import layer_norm, rms_norm
 
 pytestmark = pytest.mark.gpu
@@ -332,7 +332,7 @@ def test_weight_gradients_of_several_projections():
     x = acts(500, 200, dtype=torch.bfloat16)
     kept = keep8(x)
     gs = [torch.randn(500, n, device="cuda").bfloat16() for n in (64, 130)]
-    got = weight_grads8(gs, kept.codes, kept.scales, 200, [torch.bfloat16, torch.float32])
+    got = [weight_grad8(g, kept.codes, kept.scales, 200, dt) for g, dt in zip(gs, (torch.bfloat16, torch.float32))]
     k64 = R.kept_values(x)
     for g, t in zip(gs, got):
         g64 = g.cpu().double().t()
