@@ -70,27 +70,57 @@ __device__ __forceinline__ void store_out(void* out, int c, float v) {
 
 // ---------------------------------------------------------------- reductions
 // Sums of N values over each group of G threads; every thread of the group gets them.  `ws` holds
-// N floats a warp; calls that may overlap use different ones.
+// N floats a warp; calls that may overlap use different ones.  Inside a warp two values share each
+// exchange while there are two: a lane keeps one of a pair and hands over the other, so N values cost
+// N - 1 + log2(G) - log2(N) exchanges in place of N log2(G).
 template <int G, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float* ws) {
+  constexpr int L = G < 32 ? G : 32;
+  constexpr bool kPair = N == 2 && L >= 2;
+  const int lane = threadIdx.x & 31;
+  if constexpr (kPair) {
+    const bool odd = lane & 1;
+    float mine = odd ? v[1] : v[0];
+    mine += __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[1], 1);
 #pragma unroll
-  for (int k = 0; k < N; ++k)
+    for (int o = L / 2; o > 1; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if constexpr (G <= 32) {
+      const float other = __shfl_xor_sync(0xffffffffu, mine, 1);
+      v[0] = odd ? other : mine;
+      v[1] = odd ? mine : other;
+    } else {
+      v[0] = mine;  // even lanes: the first sum, odd lanes: the second
+    }
+  } else {
 #pragma unroll
-    for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  }
   if constexpr (G > 32) {
-    constexpr int W = G / 32;  // warps of a group
+    constexpr int W = G / 32;  // warps of a group: their sums lie together, value by value
     const int warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) {
+    float* g = ws + warp / W * W * N;
+    if constexpr (kPair) {
+      if (lane < 2) g[lane * W + warp % W] = v[0];
+    } else if (lane == 0) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) ws[warp * N + k] = v[k];
+      for (int k = 0; k < N; ++k) g[k * W + warp % W] = v[k];
     }
     __syncthreads();
-    const float* g = ws + warp / W * W * N;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       v[k] = 0.f;
+      if constexpr (W % 4 == 0) {
 #pragma unroll
-      for (int i = 0; i < W; ++i) v[k] += g[i * N + k];
+        for (int i = 0; i < W; i += 4) {
+          const float4 q = *reinterpret_cast<const float4*>(g + k * W + i);
+          v[k] += (q.x + q.y) + (q.z + q.w);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[k] += g[k * W + i];
+      }
     }
   }
 }
@@ -158,7 +188,7 @@ __global__ void __launch_bounds__(threads_of(G), CTAS)
   constexpr int NT = threads_of(G), GROUPS = NT / G;
   using X = Ring<T, NT, R * UPT>;
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ float ws[2][2][NT / 32 * R];
+  __shared__ __align__(16) float ws[2][2][NT / 32 * R];
   const int t = threadIdx.x % G, group = threadIdx.x / G;
   const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring);
   const uint64_t step = (uint64_t)gridDim.x * (GROUPS * R);
@@ -294,43 +324,42 @@ __device__ __forceinline__ void store_partial(float v, int c, int C, int which, 
   else store_out<__nv_bfloat16>(out, c, v);
 }
 
-// R rows a group a turn; dy and x (or its codes) are read from the ring twice: for the sums and dw / db, then for dx.
-template <typename T, int G, int UPT, int R, int DEPTH, int CTAS, bool LAYER, bool KEPT>
+// One row a group a turn.  Between the sums and dx a thread holds its g' and x - mean as fp32 (UPT = 2: 32
+// registers); with UPT = 4, where dw and db take the registers, it reads the ring a second time.
+template <typename T, int G, int UPT, int DEPTH, int CTAS, bool LAYER, bool KEPT>
 __global__ void __launch_bounds__(threads_of(G), CTAS)
     norm_bwd_staged_kernel(RowView dy, RowView x, Kept k, uint32_t rows, int C, Vectors vec,
                            const float* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, void* dw,
                            void* db) {
   constexpr int NT = threads_of(G), GROUPS = NT / G, N = LAYER ? 2 : 1;
-  using D = Ring<T, NT, R * UPT>;
-  using X = Ring<T, NT, R * UPT>;
-  using XK = CodeRing<NT, R * UPT>;
+  using D = Ring<T, NT, UPT>;
+  using X = Ring<T, NT, UPT>;
+  using XK = CodeRing<NT, UPT>;
   constexpr int STAGE = D::STAGE + (KEPT ? XK::STAGE : X::STAGE);
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ float ws[2][NT / 32 * N * R];
+  __shared__ __align__(16) float ws[2][NT / 32 * N];
+  constexpr bool HOLD = UPT <= 2;
   const int t = threadIdx.x % G, group = threadIdx.x / G;
   const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring);
-  const uint64_t step = (uint64_t)gridDim.x * (GROUPS * R);
-  const uint32_t first = blockIdx.x * (GROUPS * R);
+  const uint64_t step = (uint64_t)gridDim.x * (GROUPS);
+  const uint32_t first = blockIdx.x * (GROUPS);
   if (C < G * UPT * 8) zero_ring(ring, DEPTH * STAGE);
 
   auto fetch = [&](uint64_t r0, int stage) {
+    const uint64_t r = r0 + group;
+    if (r >= rows) return;
+    const uint32_t at = ring0 + stage * STAGE;
+    const T* gr = row_ptr<T>(dy, (uint32_t)r);
+    const T* xr = KEPT ? nullptr : row_ptr<T>(x, (uint32_t)r);
+    const int8_t* codes = KEPT ? k.codes + (long long)r * k.Cp : nullptr;
+    const uint8_t* scales = KEPT ? k.scales + (long long)r * k.nbp : nullptr;
 #pragma unroll
-    for (int q = 0; q < R; ++q) {
-      const uint64_t r = r0 + q * GROUPS + group;
-      if (r >= rows) continue;
-      const uint32_t at = ring0 + stage * STAGE;
-      const T* gr = row_ptr<T>(dy, (uint32_t)r);
-      const T* xr = KEPT ? nullptr : row_ptr<T>(x, (uint32_t)r);
-      const int8_t* codes = KEPT ? k.codes + (long long)r * k.Cp : nullptr;
-      const uint8_t* scales = KEPT ? k.scales + (long long)r * k.nbp : nullptr;
-#pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-        const int c = (t + i * G) * 8, slot = q * UPT + i;
-        if (c >= C) continue;
-        D::fetch(at, slot, gr + c);
-        if constexpr (KEPT) XK::fetch(at + D::STAGE, slot, codes, scales, c);
-        else X::fetch(at + D::STAGE, slot, xr + c);
-      }
+    for (int i = 0; i < UPT; ++i) {
+      const int c = (t + i * G) * 8;
+      if (c >= C) continue;
+      D::fetch(at, i, gr + c);
+      if constexpr (KEPT) XK::fetch(at + D::STAGE, i, codes, scales, c);
+      else X::fetch(at + D::STAGE, i, xr + c);
     }
   };
   // dy, and v with (x - mean) = v * unit: a layer norm subtracts the mean here (unit 1), an RMS norm leaves codes as they
@@ -370,75 +399,75 @@ __global__ void __launch_bounds__(threads_of(G), CTAS)
     }
   }
   const float inv_c = 1.f / C;
-  float2 next[R];
   auto stats_of = [&](uint64_t r0) {
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      const uint64_t r = r0 + q * GROUPS + group;
-      next[q] = r < rows ? *reinterpret_cast<const float2*>(stats + 2 * r) : make_float2(0.f, 0.f);
-    }
+    const uint64_t r = r0 + group;
+    return r < rows ? *reinterpret_cast<const float2*>(stats + 2 * r) : make_float2(0.f, 0.f);
   };
-  stats_of(first);
+  float2 next = stats_of(first);
   int stage = 0, flip = 0;
   for (uint64_t r0 = first; r0 < rows; r0 += step) {
-    float2 st[R];
-#pragma unroll
-    for (int q = 0; q < R; ++q) st[q] = next[q];
+    const float2 st = next;
     fetch(r0 + (DEPTH - 1) * step, stage == 0 ? DEPTH - 1 : stage - 1);  // into the stage of the last turn
     copy_commit();
-    stats_of(r0 + step);
+    next = stats_of(r0 + step);
     copy_wait<DEPTH - 1>();
     // with d = x - mean and g' = dy w rstd:  s = (sum g' d, sum g'),  dw += dy rstd d,  db += dy
-    float s[N * R];
+    float2 gw[HOLD ? UPT : 1][4], v[HOLD ? UPT : 1][4];
+    float unit[HOLD ? UPT : 1];
+    const uint64_t r = r0 + group;
+    const bool in = r < rows;  // a slot without a row holds another row's values
+    float2 sn = twice(0.f), sg = twice(0.f);
+    if (in) {
 #pragma unroll
-    for (int q = 0; q < R; ++q) {
-      float2 sn = twice(0.f), sg = twice(0.f);
-      if (r0 + q * GROUPS + group < rows) {  // a slot without a row holds another row's values
+      for (int i = 0; i < UPT; ++i) {
+        const int h = HOLD ? i : 0;
+        float2 g[4];
+        unit[h] = get(stage, i, (t + i * G) * 8, st.x, g, v[h]);
+        float2 part_n = twice(0.f);
 #pragma unroll
-        for (int i = 0; i < UPT; ++i) {
-          float2 g[4], v[4];
-          const float2 scale = twice(st[q].y * get(stage, q * UPT + i, (t + i * G) * 8, st[q].x, g, v));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 gr = mul2(g[j], scale);
-            const float2 gw = mul2(gr, w[i][j]);
-            sn = fma2(gw, v[j], sn);
-            aw[i][j] = fma2(gr, v[j], aw[i][j]);
-            if (LAYER) {
-              sg = add2(sg, gw);
-              ab[i][j] = add2(ab[i][j], g[j]);
-            }
+        for (int j = 0; j < 4; ++j) {
+          const float2 gr = mul2(g[j], twice(st.y));
+          gw[h][j] = mul2(gr, w[i][j]);
+          if constexpr (LAYER || !KEPT) {
+            sn = fma2(gw[h][j], v[h][j], sn);
+            aw[i][j] = fma2(gr, v[h][j], aw[i][j]);
+          } else {
+            part_n = fma2(gw[h][j], v[h][j], part_n);
+            aw[i][j] = fma2(mul2(gr, twice(unit[h])), v[h][j], aw[i][j]);
+          }
+          if (LAYER) {
+            sg = add2(sg, gw[h][j]);
+            ab[i][j] = add2(ab[i][j], g[j]);
           }
         }
+        if constexpr (!LAYER && KEPT) sn = fma2(part_n, twice(unit[h]), sn);
       }
-      s[q * N] = sn.x + sn.y;
-      if (LAYER) s[q * N + N - 1] = sg.x + sg.y;
     }
     if (dx != nullptr) {
-      group_sum<G, N * R>(s, ws[flip]);
+      float s[N];
+      s[0] = sn.x + sn.y;
+      if (LAYER) s[N - 1] = sg.x + sg.y;
+      group_sum<G, N>(s, ws[flip]);
       flip ^= 1;
-      asm volatile("" ::: "memory");  // the fragments are read from the ring again, not held in registers
-#pragma unroll
-      for (int q = 0; q < R; ++q) {
-        const uint64_t r = r0 + q * GROUPS + group;
-        if (r >= rows) continue;
+      if (in) {
         // dx = g' - mean_c(g') - d rstd^2 mean_c(g' d)
-        const float2 a = twice(LAYER ? -s[q * N + N - 1] * inv_c : 0.f);
-        const float2 b = twice(-s[q * N] * inv_c * st[q].y * st[q].y);
+        const float2 a = twice(LAYER ? -s[N - 1] * inv_c : 0.f);
+        const float b = -s[0] * inv_c * st.y * st.y;
 #pragma unroll
         for (int i = 0; i < UPT; ++i) {
-          const int c = (t + i * G) * 8;
+          const int h = HOLD ? i : 0, c = (t + i * G) * 8;
           if (c >= C) continue;
-          float2 g[4], v[4];
-          const float unit = get(stage, q * UPT + i, c, st[q].x, g, v);
-          const float2 bu = LAYER ? b : twice(b.x * unit);
+          if constexpr (!HOLD) {
+            float2 g[4];
+            unit[h] = get(stage, i, c, st.x, g, v[h]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float2 gw = mul2(mul2(g[j], twice(st[q].y)), w[i][j]);
-            if (LAYER) gw = add2(gw, a);
-            v[j] = fma2(v[j], bu, gw);
+            for (int j = 0; j < 4; ++j) gw[h][j] = mul2(mul2(g[j], twice(st.y)), w[i][j]);
           }
-          store_pairs(dx + (long long)r * C + c, v);
+          float2 o[4];
+          const float2 bu = twice(b * unit[h]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = fma2(v[h][j], bu, LAYER ? add2(gw[h][j], a) : gw[h][j]);
+          store_pairs(dx + (long long)r * C + c, o);
         }
       }
     }
@@ -475,7 +504,7 @@ __global__ void __launch_bounds__(threads_of(G), single_ctas(G))
     norm_fwd_single_kernel(RowView x, uint32_t rows, int C, Vectors vec, float eps, bool layer, T* __restrict__ y,
                            float* __restrict__ stats, Kept k) {
   constexpr int NT = threads_of(G), GROUPS = NT / G;
-  __shared__ float ws[2][2][NT / 32 * R];
+  __shared__ __align__(16) float ws[2][2][NT / 32 * R];
   const int t = threadIdx.x % G, group = threadIdx.x / G;
   float w[E], b[E];
 #pragma unroll
@@ -849,18 +878,18 @@ struct BwdCall {
   }
 };
 
-template <typename T, int G, int UPT, int R, int DEPTH, int CTAS, bool LAYER, bool KEPT>
+template <typename T, int G, int UPT, int DEPTH, int CTAS, bool LAYER, bool KEPT>
 void bwd_staged(const BwdCall& b) {
   constexpr int NT = threads_of(G), GROUPS = NT / G;
-  using D = Ring<T, NT, R * UPT>;
-  constexpr int BYTES = DEPTH * (D::STAGE + (KEPT ? CodeRing<NT, R * UPT>::STAGE : D::STAGE));
+  using D = Ring<T, NT, UPT>;
+  constexpr int BYTES = DEPTH * (D::STAGE + (KEPT ? CodeRing<NT, UPT>::STAGE : D::STAGE));
   static_assert(BYTES * CTAS <= kRingBudget, "the rings of an SM's CTAs do not fit its shared memory");
-  const int grid = grid_for(b.a.rows, GROUPS * R, CTAS);
+  const int grid = grid_for(b.a.rows, GROUPS, CTAS);
   if (b.parts != nullptr) {
     *b.parts = grid;
     return;
   }
-  const auto kernel = norm_bwd_staged_kernel<T, G, UPT, R, DEPTH, CTAS, LAYER, KEPT>;
+  const auto kernel = norm_bwd_staged_kernel<T, G, UPT, DEPTH, CTAS, LAYER, KEPT>;
   static bool ready = false;
   if (!ready) ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) == cudaSuccess;
   kernel<<<grid, NT, BYTES, b.s>>>(view_of(b.dy), view_of(b.x), kept_of(b.k), (uint32_t)b.a.rows, b.a.C, b.vec(),
@@ -904,8 +933,8 @@ void bwd_wide(const BwdCall& b) {
 template <typename T, bool LAYER, bool KEPT>
 void bwd_staged_any(const BwdCall& b) {
   const int C = b.a.C;
-  constexpr int R = sizeof(T) == 2 ? 2 : 1;
-#define STAGED(G) return bwd_staged<T, G, 2, R, 3, 2, LAYER, KEPT>(b)
+  constexpr int DEPTH = sizeof(T) == 2 ? 6 : 3;
+#define STAGED(G) return bwd_staged<T, G, 2, DEPTH, 2, LAYER, KEPT>(b)
   if (C <= 64) STAGED(4);
   if (C <= 128) STAGED(8);
   if (C <= 256) STAGED(16);
@@ -914,8 +943,8 @@ void bwd_staged_any(const BwdCall& b) {
   if (C <= 2048) STAGED(128);
   if (C <= 4096) STAGED(256);
 #undef STAGED
-  if (C <= 8192) return bwd_staged<T, 512, 2, R, 3, 1, LAYER, KEPT>(b);
-  bwd_staged<T, 512, 4, 1, sizeof(T) == 2 ? 3 : KEPT ? 2 : 1, 1, LAYER, KEPT>(b);
+  if (C <= 8192) return bwd_staged<T, 512, 2, DEPTH, 1, LAYER, KEPT>(b);
+  bwd_staged<T, 512, 4, sizeof(T) == 2 ? 3 : KEPT ? 2 : 1, 1, LAYER, KEPT>(b);
 }
 
 template <typename T, bool KEPT>
