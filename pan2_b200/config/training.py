@@ -134,6 +134,8 @@ class TrainingConfig:
     enable_gradient_checkpointing: bool = opt(True, "switch", "Recompute block activations in backward.")
     use_dedicated_gradient_checkpointing: bool = opt(False, "set", "Selective checkpointing: keep each block's attention "
                                                      "output from the forward instead of recomputing it.")
+    activation_checkpoint_bits: int = opt(16, int, "Bits of the activations kept for the backward: 8 halves block "
+                                                   "checkpoints and the caption path's activations.", choices=(16, 8))
     compile_text_encoder: bool = opt(False, "set", "Compile the text encoder (not used: eager CUDA kernels).")
     compile_transformer: bool = opt(False, "set", "Compile the transformer (not used: eager CUDA kernels).")
     compile_optimizer: bool = opt(False, "set", "Compile the optimizer (not used: fused CUDA kernels).")
@@ -196,6 +198,8 @@ class TrainingConfig:
             raise ValueError("load_transformer_weights is on but no pretrained_transformer_path is given")
         if self.load_transformer_weights and not os.path.exists(self.pretrained_transformer_path):
             raise FileNotFoundError(f"pretrained_transformer_path {self.pretrained_transformer_path} does not exist")
+        if self.activation_checkpoint_bits not in (16, 8):
+            raise ValueError(f"activation_checkpoint_bits={self.activation_checkpoint_bits!r}: 16 or 8")
         if self.gradient_accumulation_steps < 1:
             raise ValueError("gradient_accumulation_steps must be at least 1")
 

@@ -8,6 +8,10 @@ initialisation matches: ``attn_norm`` -> bias-free fused ``qkv`` -> per-head ``q
 Captions run packed (``cu_seqlens`` and host ``lens``: the varlen tcgen05 attention) or padded
 (``mask`` ``[B, L]``; the first position of every caption stays visible so an all-padding caption
 still has a key).
+
+:meth:`CaptionEncoder.set_kept8` switches the blocks to the operators that keep their activations in
+8 bits for the backward (norms, projections and the SwiGLU; the attention keeps its bf16 tensors).
+The encoder is not checkpointed, so those activations live from its forward to the end of the step.
 """
 from __future__ import annotations
 
@@ -20,6 +24,8 @@ import torch.nn.functional as F
 from .layers import RMSNorm
 from ..ops.attention import dense_attention, varlen_attention
 from ..ops.gemm import linear
+from ..ops.kept8 import kept8_linear, kept8_swiglu_ffn
+from ..ops.norm import rms_norm as fused_rms_norm
 
 
 class SwiGLUFeedForward(nn.Module):
@@ -57,6 +63,7 @@ class CaptionEncoderBlock(nn.Module):
                  eps: float = 1e-5, zero_residual_init: bool = False, residual_init_std: Optional[float] = None):
         super().__init__()
         self.heads = num_attention_heads
+        self.kept8 = False
         d_head = dim // num_attention_heads
         norm_or_id = (lambda: RMSNorm(d_head, eps=eps)) if qk_norm else nn.Identity
         self.attn_norm = RMSNorm(dim, eps=eps)
@@ -74,14 +81,28 @@ class CaptionEncoderBlock(nn.Module):
         packed = cu_seqlens is not None
         if packed and attention_mask is not None:
             raise ValueError("a caption batch is packed (cu_seqlens) or padded (attention_mask), not both")
-        h = self.attn_norm(x)
-        q, k, v = linear(h, self.qkv.weight).unflatten(-1, (3, self.heads, -1)).unbind(-3)
-        q = self.q_norm(q).to(v.dtype)
-        k = self.k_norm(k).to(v.dtype)
+        project, norm = (kept8_linear, _norm_kept8) if self.kept8 else (linear, _norm_eager)
+        h = norm(self.attn_norm, x)
+        q, k, v = project(h, self.qkv.weight).unflatten(-1, (3, self.heads, -1)).unbind(-3)
+        q = norm(self.q_norm, q).to(v.dtype)
+        k = norm(self.k_norm, k).to(v.dtype)
         o = varlen_attention(q, k, v, cu_seqlens, lens, max_seqlen) if packed else dense_attention(q, k, v,
                                                                                                   attention_mask)
-        x = x + linear(o.flatten(-2), self.attn_out.weight)
-        return x + self.ffn(self.ffn_norm(x))
+        x = x + project(o.flatten(-2), self.attn_out.weight)
+        h = norm(self.ffn_norm, x)
+        if self.kept8:
+            return x + kept8_swiglu_ffn(h, self.ffn.w1.weight, self.ffn.w3.weight, self.ffn.w2.weight)
+        return x + self.ffn(h)
+
+
+def _norm_eager(module: nn.Module, x: torch.Tensor) -> torch.Tensor:
+    return module(x)
+
+
+def _norm_kept8(module: nn.Module, x: torch.Tensor) -> torch.Tensor:
+    if isinstance(module, nn.Identity):
+        return x
+    return fused_rms_norm(x, module.weight, module.eps, kept8=True)
 
 
 class CaptionEncoder(nn.Module):
@@ -89,6 +110,11 @@ class CaptionEncoder(nn.Module):
         super().__init__()
         self.blocks = nn.ModuleList(CaptionEncoderBlock(dim=dim, num_attention_heads=num_attention_heads,
                                                         **block_kwargs) for _ in range(num_layers))
+
+    def set_kept8(self, enabled: bool = True) -> None:
+        """Keep the blocks' activations in 8 bits between forward and backward (off by default)."""
+        for block in self.blocks:
+            block.kept8 = bool(enabled)
 
     def forward(self, x, mask=None, cu_seqlens=None, lens: Optional[Sequence[int]] = None, max_seqlen=None):
         if mask is not None:

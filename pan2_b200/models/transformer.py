@@ -32,6 +32,8 @@ from .caption_encoder import CaptionEncoder
 from .packed import PackedSequenceParams
 from ..ops import packed as P
 from ..ops.gemm import linear, grouped_linear, grouped_ffn
+from ..ops.kept8 import kept8_linear
+from ..ops.norm import rms_norm as fused_rms_norm
 from ..ops.qkv import qkv_project
 from ..ops.attention import varlen_attention, dense_attention
 from ..parallel.ulysses import ulysses_attention
@@ -385,6 +387,7 @@ class PanVideoDiffusionTransformer(nn.Module):
         self.attention_backend, self.mask_text_padding = attention_backend, mask_text_padding
         self.text_embed_dim = text_embed_dim
         self.text_modulation_timestep_dependent = text_modulation_timestep_dependent
+        self.kept8 = False
         # construction order = parameter / initializer order
         self.patch_embed = VideoPatchEmbed(self.patch_size, in_channels, hidden_size)
         self.cap_embedder = nn.Sequential(RMSNorm(text_embed_dim, eps=1e-5), nn.Linear(text_embed_dim, hidden_size))
@@ -415,13 +418,24 @@ class PanVideoDiffusionTransformer(nn.Module):
         axes_dim, theta, scale = self.rope_settings()
         return rope_tables_for_grid(axes_dim, tuple(grid), theta=theta, position_scale=scale)
 
+    def set_kept8(self, enabled: bool = True) -> None:
+        """Caption path (projection of the text features and caption encoder) on the operators that keep their
+        activations in 8 bits for the backward; the joint blocks are checkpointed by the engine."""
+        self.kept8 = bool(enabled)
+        self.caption_encoder.set_kept8(enabled)
+
+    def _embed_captions(self, text_states):
+        norm, proj = self.cap_embedder
+        if self.kept8:
+            return kept8_linear(fused_rms_norm(text_states, norm.weight, norm.eps, kept8=True), proj.weight, proj.bias)
+        return linear(rms_norm(text_states, norm.weight.to(text_states.dtype), norm.eps), proj.weight, proj.bias)
+
     # ------------------------------------------------------------------ packed (training)
     def embed_packed(self, hidden_states, timestep, text_states, meta: PackedSequenceParams):
         """Everything before the joint blocks: returns ``(x, ln_stats, vec)``."""
         vec = self.timestep_encoder(timestep)
         vec = vec.to(hidden_states.dtype) if hidden_states.is_floating_point() else vec
-        txt = linear(rms_norm(text_states, self.cap_embedder[0].weight.to(text_states.dtype), self.cap_embedder[0].eps),
-                     self.cap_embedder[1].weight, self.cap_embedder[1].bias)
+        txt = self._embed_captions(text_states)
         cap_lens = meta.cp_caption_lens if meta.cp_caption_lens is not None else meta.caption_lens
         txt = self.caption_encoder(txt, cu_seqlens=meta.caption_cu_seqlens, lens=cap_lens,
                                    max_seqlen=meta.caption_segment_limit)
@@ -497,8 +511,7 @@ class PanVideoDiffusionTransformer(nn.Module):
 
     def encode_text(self, text_states, text_mask):
         mask = text_mask if self.mask_text_padding else None
-        t = linear(rms_norm(text_states, self.cap_embedder[0].weight.to(text_states.dtype), self.cap_embedder[0].eps),
-                   self.cap_embedder[1].weight, self.cap_embedder[1].bias)
+        t = self._embed_captions(text_states)
         t = self.caption_encoder(t, mask=mask)
         if self.text_type_embedding is not None:
             t = t + self.text_type_embedding.vector.to(t.dtype)

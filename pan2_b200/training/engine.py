@@ -33,6 +33,7 @@ import torch.nn as nn
 from ..models.transformer import PanVideoDiffusionTransformer, JointAttentionBlock
 from ..models.packed import PackedSequenceParams
 from ..ops._ext import ext
+from ..ops.kept8 import Kept8, keep8, restore8
 from ..optim import flat_ops as F
 from ..optim.muon import adjust_lr_scale, chunk_view, gram_newton_schulz
 from ..parallel.collectives import all_to_all_list
@@ -104,7 +105,12 @@ class BlockCheckpoint(torch.autograd.Function):
         sm.release(u)
         ctx.engine, ctx.idx = engine, idx
         stash = engine.stash_checkpoint(idx, x, ln_stats)
-        if stash is None:
+        ctx.kept = None
+        if stash is None and engine.checkpoint_bits == 8:
+            kept = keep8(x)
+            ctx.save_for_backward(kept.codes, kept.scales, ln_stats, vec)
+            ctx.kept, ctx.stash = (kept.shape, kept.dtype), None
+        elif stash is None:
             ctx.save_for_backward(x, ln_stats, vec)
             ctx.stash = None
         else:
@@ -118,7 +124,10 @@ class BlockCheckpoint(torch.autograd.Function):
         engine, idx = ctx.engine, ctx.idx
         sm = engine.sharded
         u = sm.units[idx]
-        if ctx.stash is None:
+        if ctx.kept is not None:
+            codes, scales, ln_stats, vec = ctx.saved_tensors
+            x = restore8(Kept8(codes, scales, *ctx.kept))
+        elif ctx.stash is None:
             x, ln_stats, vec = ctx.saved_tensors
         else:
             (vec,) = ctx.saved_tensors
@@ -338,6 +347,7 @@ class TrainEngine:
         # activation checkpointing of the joint blocks (set_activation_checkpointing)
         self.recompute_blocks = True
         self.keep_attention = False
+        self.checkpoint_bits = 16
         self._kept_attn: Dict[int, tuple] = {}
         self.accum_steps = 1
         self.accumulating = False
@@ -452,12 +462,21 @@ class TrainEngine:
             raise ValueError("keeping attention outputs (use_dedicated_gradient_checkpointing) is not supported "
                              "with context parallelism (cp_size > 1)")
 
-    def set_activation_checkpointing(self, enabled: bool = True, keep_attention: bool = False) -> None:
+    def set_activation_checkpointing(self, enabled: bool = True, keep_attention: bool = False, bits: int = 16) -> None:
         """``enabled``: recompute each joint block's forward before its backward (the default);
         off, every block keeps its activations.  ``keep_attention``: selective checkpointing that
         keeps each block's attention output and log-sum-exp from the forward, so the recompute skips
         the attention forward (about 0.8 GB per block at 95k tokens of the 29B model); the QKV
-        projection is still recomputed (reference: train.py:817-845)."""
+        projection is still recomputed (reference: train.py:817-845).
+
+        ``bits=8`` keeps activations in 8 bits (:mod:`pan2_b200.ops.kept8`): block checkpoints that take
+        memory of their own (those parked in idle gradient buffers stay as they are: they are free and
+        exact), and the caption path's norm, projection and SwiGLU inputs.  The forward is exact up to the
+        fused norms' single rounding; gradients carry the store's error (about 1 % of a block's values)."""
+        if bits not in (8, 16):
+            raise ValueError(f"activations are kept in 16 or 8 bits, not {bits}")
+        self.checkpoint_bits = bits
+        self.model.set_kept8(bits == 8)
         self.recompute_blocks = bool(enabled)
         self.keep_attention = bool(keep_attention) and self.recompute_blocks
         if self.keep_attention and getattr(self, "cp_size", 1) > 1:

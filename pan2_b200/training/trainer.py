@@ -140,7 +140,8 @@ class Trainer:
                                   seed=cfg.seed, optim=optim, offload=cfg.optimizer_offload,
                                   activation_bytes_estimate=act, replicate_group=L.replicate_group)
         self.engine.set_activation_checkpointing(cfg.enable_gradient_checkpointing,
-                                                 cfg.use_dedicated_gradient_checkpointing)
+                                                 cfg.use_dedicated_gradient_checkpointing,
+                                                 cfg.activation_checkpoint_bits)
         if cfg.cp_size > 1:
             self.engine.set_context_parallel(L.cp_group, L.cp_size, L.cp_rank)
         self.engine.set_accumulation(cfg.gradient_accumulation_steps)
@@ -402,7 +403,8 @@ class Trainer:
             log.info(f"Training for {cfg.max_steps} steps: batch_size={cfg.batch_size} (packed batches are sized "
                      f"by the token budgets) lr={cfg.learning_rate} weight_decay={cfg.weight_decay} "
                      f"zero_init_modulation={cfg.zero_init_modulation} activation_checkpointing="
-                     f"{'kept-attention' if self.engine.keep_attention else cfg.enable_gradient_checkpointing}")
+                     f"{'kept-attention' if self.engine.keep_attention else cfg.enable_gradient_checkpointing}"
+                     f"{', 8-bit' if cfg.activation_checkpoint_bits == 8 else ''}")
         loader = None
         it = None
         if not self.layout.cp_enabled or self.layout.cp_rank == 0:
