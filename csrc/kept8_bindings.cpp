@@ -67,7 +67,8 @@ RowsOf rows_of(torch::Tensor t, const char* name) {
       ++levels;
     }
     if (levels <= 2 || attempt == 1) {
-      if (levels <= 1) r.a = RowsArg{t.data_ptr(), stride[0], 0, 1};
+      if (levels == 0) r.a = RowsArg{t.data_ptr(), r.C, 0, 1};
+      else if (levels == 1) r.a = RowsArg{t.data_ptr(), stride[0], 0, 1};
       else r.a = RowsArg{t.data_ptr(), stride[1], stride[0], size[0]};
       break;
     }
@@ -95,7 +96,9 @@ Kept8Buf kept_of(const torch::Tensor& codes, const torch::Tensor& scales, int64_
                   scales.dim() == 2 && scales.size(0) == rows && scales.size(1) == kept_scales(C) &&
                   scales.device() == codes.device(),
               "kept scales must be contiguous uint8 [rows, blocks rounded up to 4] beside the codes");
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0, "kept codes must be 16-byte aligned");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
+              "kept codes and scales must be 16-byte aligned");
   return Kept8Buf{codes.data_ptr(), scales.data_ptr(), (int)C};
 }
 
@@ -151,7 +154,8 @@ void restore8(torch::Tensor codes, torch::Tensor scales, int64_t C, int64_t row0
               "restore8: out must be a row-major bf16 or fp32 [rows, >= C] CUDA matrix");
   TORCH_CHECK(row0 >= 0 && row0 + out.size(0) <= codes.size(0) && codes.size(0) < (1ll << 31),
               "restore8: rows out of range");
-  launch_restore8(k, row0, out.size(0), out.scalar_type() == torch::kFloat32, out.data_ptr(), out.stride(0), stream());
+  launch_restore8(k, row0, out.size(0), out.scalar_type() == torch::kFloat32, out.data_ptr(), out.stride(0), (int)C,
+                  stream());
   check_launch(nullptr, "restore8");
 }
 
@@ -311,8 +315,7 @@ torch::Tensor weight_grad8(const torch::Tensor& gp, int64_t N, const torch::Tens
   auto x = torch::empty({one ? rows : kWgradRows, up8(K)}, gp.options());
   for (int64_t r0 = 0; r0 < rows; r0 += kWgradRows) {
     const int64_t n = std::min(kWgradRows, rows - r0);
-    // padding columns of x only reach padding columns of the result
-    launch_restore8(k, r0, n, false, x.data_ptr(), x.size(1), stream());
+    launch_restore8(k, r0, n, false, x.data_ptr(), x.size(1), (int)x.size(1), stream());
     gemm(gp.narrow(0, r0, n), x.narrow(0, 0, n), out, false, false, c10::nullopt, c10::nullopt, r0 > 0);
   }
   check_launch(nullptr, "weight_grad8");

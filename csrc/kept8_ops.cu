@@ -1,9 +1,12 @@
 // 8-bit kept activations (sm_100a): store, reload, the SwiGLU whose gate and value are kept in 8 bits,
 // and the column sums that its neighbours' bias gradients need.  The format is in kept8.cuh.
 //
-// All kernels here are element streams bounded by DRAM.  Work is cut into fragments of V elements
-// (V = 8 when every row is 16-byte aligned and C % 8 == 0, V = 1 otherwise); the 32 / V lanes that
-// hold one block of 32 agree on its scale by shuffles, so every input is read once.
+// All kernels here are element streams bounded by DRAM.  Work is cut into fragments of V elements; the 32 / V lanes
+// that hold one block of 32 agree on its scale by shuffles, so every input is read once.  Three forms:
+//   V = 8   C % 8 == 0 and every row 16-byte aligned: 16-byte accesses
+//   flat    contiguous tensors of any other width: tiles through shared memory (flat.cuh), V = 4 there
+//   V = 1   what is left (odd views): one element a lane
+#include "flat.cuh"
 #include "kept8.cuh"
 #include "launchers.h"
 
@@ -231,6 +234,213 @@ __global__ void __launch_bounds__(kThreads) swiglu_bwd_kernel(RowView dh, Kept8O
   }
 }
 
+// ---------------------------------------------------------------- flat form
+// A tile is kFlatTile elements of whole rows, or of one row when that is longer.  Lane groups of eight hold a block, four
+// elements a lane; a tile's fragments are (row, 4 columns) over rows padded to whole blocks.
+constexpr int kFlatTile = 4096;
+
+struct FlatTiles {
+  FastDiv per_row, frag_row;  // tiles a row (1 unless rows are long), fragments a padded row of a tile
+  int rows, C;                // rows a tile
+  uint32_t total_rows;
+};
+
+struct FlatTile {
+  uint32_t row0, rows;
+  int c0, cols;      // columns c0 .. c0 + cols of every row
+  uint32_t frags;    // fragments of the tile
+};
+
+__device__ __forceinline__ FlatTile flat_tile(const FlatTiles& t) {
+  FlatTile f;
+  if (t.rows > 1 || t.per_row.d == 1) {
+    f.row0 = blockIdx.x * t.rows;
+    f.rows = min((uint32_t)t.rows, t.total_rows - f.row0);
+    f.c0 = 0;
+    f.cols = t.C;
+  } else {
+    f.row0 = t.per_row.div(blockIdx.x);
+    f.rows = 1;
+    f.c0 = (int)(blockIdx.x - f.row0 * t.per_row.d) * kFlatTile;
+    f.cols = min(kFlatTile, t.C - f.c0);
+  }
+  f.frags = f.rows * ((f.cols + kKeptBlock - 1) / kKeptBlock * (kKeptBlock / 4));
+  return f;
+}
+
+// Fragment u of the tile: its row (in the tile) and first column (in the tile).
+__device__ __forceinline__ void flat_frag(const FlatTiles& t, const FlatTile& f, uint32_t u, uint32_t& r, int& c) {
+  r = f.rows == 1 ? 0 : t.frag_row.div(u);
+  c = (int)(u - r * t.frag_row.d) * 4;
+}
+
+template <typename T>
+__device__ __forceinline__ void flat_read(const uint8_t* smem, const FlatTile& f, uint32_t r, int c, float (&v)[4]) {
+  const T* p = reinterpret_cast<const T*>(smem) + r * f.cols + c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = c + i < f.cols ? to_f32(p[i]) : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void flat_write(uint8_t* smem, const FlatTile& f, uint32_t r, int c, const float (&v)[4]) {
+  T* p = reinterpret_cast<T*>(smem) + r * f.cols + c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (c + i < f.cols) p[i] = from_f32<T>(v[i]);
+}
+
+// Scale and codes of a fragment; all lanes of the warp take part, `act` lanes store.
+__device__ __forceinline__ void flat_keep(const Kept8Out& o, uint32_t row, int c, bool act, const float (&v)[4]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  const uint32_t b = kept8_byte(m);
+  if (!act) return;
+  const float inv = kept8_inv_step(b);
+  *reinterpret_cast<uint32_t*>(o.codes + (long long)row * o.Cp + c) =
+      pack4_low_bytes(kept8_code(v[0], inv), kept8_code(v[1], inv), kept8_code(v[2], inv), kept8_code(v[3], inv));
+  if (c % kKeptBlock == 0) kept8_store_byte(o.scales + (long long)row * o.nbp, c / kKeptBlock, o.nb, o.nbp, b);
+}
+
+__device__ __forceinline__ void flat_values(const Kept8Out& k, uint32_t row, int c, float (&v)[4]) {
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(k.codes + (long long)row * k.Cp + c) ^ 0x80808080u;
+  const float step = kept8_step(k.scales[(long long)row * k.nbp + c / kKeptBlock]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 + i)) - 8388736.f) * step;
+}
+
+template <typename T>
+constexpr uint32_t flat_room() { return FlatRun<T>::room(kFlatTile); }
+__device__ __forceinline__ void flat_wait() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+}
+template <typename T>
+__device__ __forceinline__ FlatRun<T> flat_run(const void* p, const FlatTiles& t, const FlatTile& f) {
+  return FlatRun<T>(p, (long long)f.row0 * t.C + f.c0, f.rows * (uint32_t)f.cols);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) keep8_flat_kernel(const T* x, FlatTiles t, Kept8Out o, T* __restrict__ copy,
+                                                              long long ld) {
+  __shared__ __align__(16) uint8_t sx[flat_room<T>()];
+  const FlatTile f = flat_tile(t);
+  const FlatRun<T> run = flat_run<T>(x, t, f);
+  run.fetch(sx);
+  flat_wait();
+  for (uint32_t u0 = 0; u0 < f.frags; u0 += kThreads) {  // whole warps: a tile's fragments are a multiple of 8
+    const uint32_t u = u0 + threadIdx.x;
+    const bool act = u < f.frags;
+    uint32_t r;
+    int c;
+    flat_frag(t, f, act ? u : 0, r, c);
+    float v[4];
+    flat_read<T>(sx + run.head, f, r, c, v);
+    const uint32_t row = f.row0 + r;
+    flat_keep(o, row, f.c0 + c, act, v);
+    if constexpr (sizeof(T) == 2) {
+      if (copy != nullptr && act && f.c0 + c < ld)  // ld % 8 == 0: the four columns are inside
+        *reinterpret_cast<uint2*>(copy + (long long)row * ld + f.c0 + c) =
+            make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) restore8_flat_kernel(FlatTiles t, Kept8Out k, T* __restrict__ out) {
+  __shared__ __align__(16) uint8_t so[flat_room<T>()];
+  const FlatTile f = flat_tile(t);
+  const FlatRun<T> run = flat_run<T>(out, t, f);
+#pragma unroll 2
+  for (uint32_t u = threadIdx.x; u < f.frags; u += kThreads) {
+    uint32_t r;
+    int c;
+    flat_frag(t, f, u, r, c);
+    float v[4];
+    flat_values(k, f.row0 + r, f.c0 + c, v);
+    flat_write<T>(so + run.head, f, r, c, v);
+  }
+  __syncthreads();
+  run.store(so);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) swiglu_fwd_flat_kernel(const T* gate, const T* value, FlatTiles t,
+                                                                   Kept8Out og, Kept8Out ov, T* __restrict__ h) {
+  __shared__ __align__(16) uint8_t sg[flat_room<T>()], sv[flat_room<T>()];
+  const FlatTile f = flat_tile(t);
+  const FlatRun<T> rg = flat_run<T>(gate, t, f), rv = flat_run<T>(value, t, f), rh = flat_run<T>(h, t, f);
+  rg.fetch(sg);
+  rv.fetch(sv);
+  flat_wait();
+  for (uint32_t u0 = 0; u0 < f.frags; u0 += kThreads) {
+    const uint32_t u = u0 + threadIdx.x;
+    const bool act = u < f.frags;
+    uint32_t r;
+    int c;
+    flat_frag(t, f, act ? u : 0, r, c);
+    float g[4], v[4];
+    flat_read<T>(sg + rg.head, f, r, c, g);
+    flat_read<T>(sv + rv.head, f, r, c, v);
+    if (og.codes != nullptr) {
+      flat_keep(og, f.row0 + r, f.c0 + c, act, g);
+      flat_keep(ov, f.row0 + r, f.c0 + c, act, v);
+    }
+    if (!act) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] *= g[i] * sigmoid_fast(g[i]);
+    flat_write<T>(sv + rv.head, f, r, c, v);  // h takes the place of value: same offsets, own elements
+  }
+  __syncthreads();
+  rh.store(sv);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) swiglu_bwd_flat_kernel(const T* dh, Kept8Out kg, Kept8Out kv, FlatTiles t,
+                                                                   T* __restrict__ dgate, T* __restrict__ dvalue,
+                                                                   T* __restrict__ h) {
+  __shared__ __align__(16) uint8_t sd[flat_room<T>()], sv[flat_room<T>()];
+  const FlatTile f = flat_tile(t);
+  const FlatRun<T> rd = flat_run<T>(dh, t, f);
+  rd.fetch(sd);
+  flat_wait();
+  for (int pass = 0; pass < (h != nullptr ? 2 : 1); ++pass) {  // dgate over dh and dvalue; then h by itself
+    for (uint32_t u = threadIdx.x; u < f.frags; u += kThreads) {
+      uint32_t r;
+      int c;
+      flat_frag(t, f, u, r, c);
+      float g[4], w[4];
+      flat_values(kg, f.row0 + r, f.c0 + c, g);
+      flat_values(kv, f.row0 + r, f.c0 + c, w);
+      if (pass == 0) {
+        float d[4], o[4];
+        flat_read<T>(sd + rd.head, f, r, c, d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float s = sigmoid_fast(g[i]), ds = d[i] * s;
+          o[i] = ds * w[i] * fmaf(g[i], 1.f - s, 1.f);
+          d[i] = ds * g[i];
+        }
+        flat_write<T>(sd + rd.head, f, r, c, o);
+        flat_write<T>(sv + rd.head, f, r, c, d);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] *= g[i] * sigmoid_fast(g[i]);
+        flat_write<T>(sd + rd.head, f, r, c, w);
+      }
+    }
+    __syncthreads();
+    if (pass == 0) {
+      flat_run<T>(dgate, t, f).store(sd);
+      flat_run<T>(dvalue, t, f).store(sv);
+      __syncthreads();
+    } else {
+      flat_run<T>(h, t, f).store(sd);
+    }
+  }
+}
+
 // ---------------------------------------------------------------- column sums
 // A CTA sums a chunk of rows of 256 / TR column fragments, TR rows at a time; part[chunk, c] then goes to a second
 // kernel unless there is one chunk.  A fixed order, no atomics.
@@ -317,9 +527,10 @@ void keep8_t(const RowsArg& x, long long rows, const Kept8Buf& k, void* copy, lo
 }
 
 template <typename T, int V>
-void restore8_t(const Kept8Buf& k, long long row0, long long rows, void* out, long long ld, cudaStream_t s) {
+void restore8_t(const Kept8Buf& k, long long row0, long long rows, void* out, long long ld, int cols, cudaStream_t s) {
   constexpr int U = V == 1 ? 8 : 4;
   Kept8Out o = out_of(k);
+  o.C = cols;
   o.codes += row0 * o.Cp;
   o.scales += row0 * o.nbp;
   over_rows<V, U>(rows, o.Cp, [&](const Units& un, uint32_t grid) {
@@ -347,6 +558,25 @@ void swiglu_bwd_t(const RowsArg& dh, long long rows, const Kept8Buf& kg, const K
   });
 }
 
+// Whether `a` is a contiguous, 16-byte aligned tensor of rows of C.
+bool contiguous_rows(const RowsArg& a, int C) {
+  return a.inner == 1 && a.outer_stride == C && reinterpret_cast<uintptr_t>(a.p) % 16 == 0;
+}
+
+FlatTiles flat_tiles(long long rows, int C, uint32_t* grid) {
+  FlatTiles t;
+  const int tiles = (C + kFlatTile - 1) / kFlatTile;
+  t.per_row = FastDiv((uint32_t)tiles);
+  t.rows = tiles > 1 ? 1 : kFlatTile / C;
+  t.C = C;
+  t.frag_row = FastDiv((uint32_t)((tiles > 1 ? kFlatTile : (C + kKeptBlock - 1) / kKeptBlock * kKeptBlock) / 4));
+  t.total_rows = (uint32_t)rows;
+  *grid = tiles > 1 ? (uint32_t)rows * (uint32_t)tiles : (uint32_t)((rows + t.rows - 1) / t.rows);
+  return t;
+}
+// Tiles are counted in 31 bits.
+bool flat_fits(long long rows, int C) { return rows * ((C + kFlatTile - 1) / kFlatTile) < (1ll << 31); }
+
 // 16-byte fragments: C in whole fragments and every row start aligned.
 bool fragments_of_8(const RowsArg& a, int C, bool fp32) {
   const int e = fp32 ? 4 : 2;
@@ -369,17 +599,36 @@ bool fragments_of_8(const RowsArg& a, int C, bool fp32) {
 void launch_keep8(const RowsArg& x, long long rows, bool fp32, const Kept8Buf& k, void* copy, long long ld,
                   cudaStream_t s) {
   if (rows <= 0) return;
+  const bool vec = fragments_of_8(x, k.C, fp32);
+  if (!vec && contiguous_rows(x, k.C) && flat_fits(rows, k.C)) {
+    uint32_t grid;
+    const FlatTiles t = flat_tiles(rows, k.C, &grid);
+    if (fp32) keep8_flat_kernel<float><<<grid, kThreads, 0, s>>>((const float*)x.p, t, out_of(k), (float*)copy, ld);
+    else keep8_flat_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>((const __nv_bfloat16*)x.p, t, out_of(k), (__nv_bfloat16*)copy, ld);
+    return;
+  }
 #define CALL(T, V) keep8_t<T, V>(x, rows, k, copy, ld, s)
-  PAN_BY_TYPE(fp32, fragments_of_8(x, k.C, fp32), CALL);
+  PAN_BY_TYPE(fp32, vec, CALL);
 #undef CALL
 }
 
-void launch_restore8(const Kept8Buf& k, long long row0, long long rows, bool fp32, void* out, long long ld,
+void launch_restore8(const Kept8Buf& k, long long row0, long long rows, bool fp32, void* out, long long ld, int cols,
                      cudaStream_t s) {
   if (rows <= 0) return;
   const RowsArg o{out, ld, 0, 1};
-#define CALL(T, V) restore8_t<T, V>(k, row0, rows, out, ld, s)
-  PAN_BY_TYPE(fp32, fragments_of_8(o, k.C, fp32), CALL);
+  const bool vec = fragments_of_8(o, cols, fp32);
+  if (!vec && cols == k.C && contiguous_rows(o, k.C) && flat_fits(rows, k.C)) {
+    uint32_t grid;
+    const FlatTiles t = flat_tiles(rows, k.C, &grid);
+    Kept8Out from = out_of(k);
+    from.codes += row0 * from.Cp;
+    from.scales += row0 * from.nbp;
+    if (fp32) restore8_flat_kernel<float><<<grid, kThreads, 0, s>>>(t, from, (float*)out);
+    else restore8_flat_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(t, from, (__nv_bfloat16*)out);
+    return;
+  }
+#define CALL(T, V) restore8_t<T, V>(k, row0, rows, out, ld, cols, s)
+  PAN_BY_TYPE(fp32, vec, CALL);
 #undef CALL
 }
 
@@ -387,6 +636,17 @@ void launch_swiglu_fwd(const RowsArg& g, const RowsArg& v, long long rows, bool 
                        const Kept8Buf& kv, void* h, cudaStream_t s) {
   if (rows <= 0) return;
   const bool vec = fragments_of_8(g, kg.C, fp32) && fragments_of_8(v, kg.C, fp32);
+  if (!vec && contiguous_rows(g, kg.C) && contiguous_rows(v, kg.C) && flat_fits(rows, kg.C)) {
+    uint32_t grid;
+    const FlatTiles t = flat_tiles(rows, kg.C, &grid);
+    if (fp32)
+      swiglu_fwd_flat_kernel<float><<<grid, kThreads, 0, s>>>((const float*)g.p, (const float*)v.p, t, out_of(kg),
+                                                              out_of(kv), (float*)h);
+    else
+      swiglu_fwd_flat_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(
+          (const __nv_bfloat16*)g.p, (const __nv_bfloat16*)v.p, t, out_of(kg), out_of(kv), (__nv_bfloat16*)h);
+    return;
+  }
 #define CALL(T, V) swiglu_fwd_t<T, V>(g, v, rows, kg, kv, h, s)
   PAN_BY_TYPE(fp32, vec, CALL);
 #undef CALL
@@ -395,8 +655,21 @@ void launch_swiglu_fwd(const RowsArg& g, const RowsArg& v, long long rows, bool 
 void launch_swiglu_bwd(const RowsArg& dh, long long rows, bool fp32, const Kept8Buf& kg, const Kept8Buf& kv, void* dg,
                        void* dv, void* h, cudaStream_t s) {
   if (rows <= 0) return;
+  const bool vec = fragments_of_8(dh, kg.C, fp32);
+  if (!vec && contiguous_rows(dh, kg.C) && flat_fits(rows, kg.C)) {
+    uint32_t grid;
+    const FlatTiles t = flat_tiles(rows, kg.C, &grid);
+    if (fp32)
+      swiglu_bwd_flat_kernel<float><<<grid, kThreads, 0, s>>>((const float*)dh.p, out_of(kg), out_of(kv), t, (float*)dg,
+                                                              (float*)dv, (float*)h);
+    else
+      swiglu_bwd_flat_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>((const __nv_bfloat16*)dh.p, out_of(kg), out_of(kv),
+                                                                      t, (__nv_bfloat16*)dg, (__nv_bfloat16*)dv,
+                                                                      (__nv_bfloat16*)h);
+    return;
+  }
 #define CALL(T, V) swiglu_bwd_t<T, V>(dh, rows, kg, kv, dg, dv, h, s)
-  PAN_BY_TYPE(fp32, fragments_of_8(dh, kg.C, fp32), CALL);
+  PAN_BY_TYPE(fp32, vec, CALL);
 #undef CALL
 }
 

@@ -46,8 +46,9 @@ void launch_keep8(const RowsArg& x, long long rows, bool fp32, const Kept8Buf& k
                   cudaStream_t s);
 // out [rows, ld] bf16 = x [rows, C], zeros past C (ld = C rounded up to 8).
 void launch_pad_rows(const RowsArg& x, long long rows, int C, void* out, long long ld, cudaStream_t s);
-// Rows row0 .. row0 + rows of `k` into out (row stride ld).
-void launch_restore8(const Kept8Buf& k, long long row0, long long rows, bool fp32, void* out, long long ld,
+// Rows row0 .. row0 + rows of `k` into out (row stride ld): `cols` columns, C or more (zeros past C) and at most
+// the codes' padded width.
+void launch_restore8(const Kept8Buf& k, long long row0, long long rows, bool fp32, void* out, long long ld, int cols,
                      cudaStream_t s);
 void launch_swiglu_fwd(const RowsArg& g, const RowsArg& v, long long rows, bool fp32, const Kept8Buf& kg,
                        const Kept8Buf& kv, void* h, cudaStream_t s);

@@ -11,11 +11,13 @@
 // Both directions are DRAM-bound, so every tensor is read and written once.  A group of G threads owns the
 // columns of a row for all the rows that its CTA walks: weight, bias and the growing dw / db stay in
 // registers, and one partial row of dw / db per CTA goes to scratch, which a second kernel adds up in order (no
-// atomics: the same bits every time).  Three forms:
+// atomics: the same bits every time).  Four forms:
 //   staged   (C % 8 == 0, 16-byte aligned rows, C <= 16384)  8-column fragments through rings in shared memory
-//   single   (any other rows up to 16384 / 8192 columns)     one column at a time, rows in registers
+//   flat     (contiguous rows of other widths, C <= 8192)    batches of rows as one run of bytes (flat.cuh)
+//   single   (other views, C <= 8192)                        one column at a time, straight from memory
 //   wide     (wider rows)                                    CTA per row, the row swept from memory
 // Groups of up to a warp reduce by shuffles, larger ones through shared memory.
+#include "flat.cuh"
 #include "kept8.cuh"
 #include "launchers.h"
 
@@ -495,10 +497,269 @@ __global__ void __launch_bounds__(threads_of(G), CTAS)
   }
 }
 
+// ---------------------------------------------------------------- flat form
+// A batch is GROUPS * R neighbouring rows, one run of bytes; the next two or three arrive while one is worked on (one
+// ahead left the kernel waiting for memory at 35 % of its bandwidth).  Fragment i of thread t are the 4 columns from 4 (t + i G) on: eight lanes hold a block of
+// the codes.  Results take the place of the input and leave as one run.
+constexpr int flat_ctas(int G, int R) { return threads_of(G) > 256 ? 1 : R == 1 ? 3 : 2; }
+constexpr int flat_depth(int G) { return threads_of(G) <= 512 ? 4 : 3; }
+constexpr int kFlatUpt = 2;
+
+template <typename T, int G, int R>
+struct FlatBatch {
+  static constexpr int NT = threads_of(G), GROUPS = NT / G, ROWS = GROUPS * R, WIDTH = G * kFlatUpt * 4;
+  static constexpr uint32_t ROOM = FlatRun<T>::room(ROWS * WIDTH);
+  static constexpr uint32_t CODES = FlatRun<int8_t>::room(ROWS * WIDTH), SCALES = FlatRun<uint8_t>::room(ROWS * (WIDTH / kKeptBlock));
+};
+
+// `n` of the four elements from p on, zeros for the others.
+template <typename T>
+__device__ __forceinline__ void read4(const T* p, int n, float (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = j < n ? to_f32(p[j]) : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void write4(T* p, int n, const float (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < n) p[j] = from_f32<T>(v[j]);
+}
+
+template <typename T, int G, int R>
+__global__ void __launch_bounds__(threads_of(G), flat_ctas(G, R))
+    norm_fwd_flat_kernel(const T* x, uint32_t rows, int C, Vectors vec, float eps, bool layer, T* __restrict__ y,
+                         float* __restrict__ stats, Kept k) {
+  using B = FlatBatch<T, G, R>;
+  constexpr int UPT = kFlatUpt;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ __align__(16) float ws[2][2][B::NT / 32 * R];
+  const int t = threadIdx.x % G, group = threadIdx.x / G;
+  auto run_of = [&](const T* p, uint64_t r0) {
+    return FlatRun<T>(p, (long long)r0 * C, (uint32_t)min((uint64_t)B::ROWS, rows - r0) * C);
+  };
+  const uint64_t step = (uint64_t)gridDim.x * B::ROWS;
+  uint64_t r0 = (uint64_t)blockIdx.x * B::ROWS;
+  constexpr int DEPTH = flat_depth(G);
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; ++d) {
+    if (r0 + d * step < rows) run_of(x, r0 + d * step).fetch(ring + d * B::ROOM);
+    copy_commit();
+  }
+  float w[UPT][4], b[UPT][4];
+  int n[UPT];  // columns of the fragment inside the row
+#pragma unroll
+  for (int i = 0; i < UPT; ++i) {
+    const int c = (t + i * G) * 4;
+    n[i] = max(0, min(4, C - c));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[i][j] = j < n[i] ? vec_at(vec.w, vec.fp32, c + j, 1.f) : 0.f;
+      b[i][j] = j < n[i] ? vec_at(vec.b, vec.fp32, c + j, 0.f) : 0.f;
+    }
+  }
+  const float inv_c = 1.f / C;
+  int stage = 0, flip = 0;
+  for (; r0 < rows; r0 += step, stage = stage == DEPTH - 1 ? 0 : stage + 1, flip ^= 1) {
+    const uint64_t ahead = r0 + (DEPTH - 1) * step;
+    if (ahead < rows) run_of(x, ahead).fetch(ring + (stage == 0 ? DEPTH - 1 : stage - 1) * B::ROOM);
+    copy_commit();
+    copy_wait<DEPTH - 1>();
+    __syncthreads();
+    T* tile = reinterpret_cast<T*>(ring + stage * B::ROOM + run_of(x, r0).head);
+    float v[R][UPT][4], mean[R], var[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const int row = q * B::GROUPS + group;
+      const bool in = r0 + row < rows;
+      mean[q] = 0.f;
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        read4(tile + row * C + (t + i * G) * 4, in ? n[i] : 0, v[q][i]);
+        mean[q] += (v[q][i][0] + v[q][i][1]) + (v[q][i][2] + v[q][i][3]);
+      }
+    }
+    if (layer) group_sum<G, R>(mean, ws[flip][0]);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      mean[q] = layer ? mean[q] * inv_c : 0.f;
+      var[q] = 0.f;
+#pragma unroll
+      for (int i = 0; i < UPT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float d = j < n[i] ? v[q][i][j] - mean[q] : 0.f;
+          var[q] = fmaf(d, d, var[q]);
+        }
+    }
+    group_sum<G, R>(var, ws[flip][1]);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const int row = q * B::GROUPS + group;
+      const uint64_t r = r0 + row;
+      if (r >= rows) continue;  // the whole group
+      const float rstd = rsqrtf(var[q] * inv_c + eps);
+      if (t == 0 && stats != nullptr) *reinterpret_cast<float2*>(stats + 2 * r) = make_float2(mean[q], rstd);
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        const int c = (t + i * G) * 4;
+        if (k.codes != nullptr) {
+          uint32_t m = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(v[q][i][j]) & 0x7fffffffu);
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+          const uint32_t sb = kept8_byte(m);
+          if (c < k.Cp) {
+            const float inv = kept8_inv_step(sb);
+            *reinterpret_cast<uint32_t*>(k.codes + (long long)r * k.Cp + c) =
+                pack4_low_bytes(kept8_code(v[q][i][0], inv), kept8_code(v[q][i][1], inv), kept8_code(v[q][i][2], inv),
+                                kept8_code(v[q][i][3], inv));
+            if (c % kKeptBlock == 0) kept8_store_byte(k.scales + (long long)r * k.nbp, c / kKeptBlock, k.nb, k.nbp, sb);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[q][i][j] = fmaf((v[q][i][j] - mean[q]) * rstd, w[i][j], b[i][j]);
+        write4(tile + row * C + c, n[i], v[q][i]);
+      }
+    }
+    __syncthreads();
+    run_of(y, r0).store(ring + stage * B::ROOM);  // y is aligned as x is: the same offsets
+    __syncthreads();
+  }
+}
+
+template <typename T, int G, int R, bool KEPT>
+__global__ void __launch_bounds__(threads_of(G), flat_ctas(G, R))
+    norm_bwd_flat_kernel(const T* dy, const T* x, Kept k, uint32_t rows, int C, Vectors vec, bool layer,
+                         const float* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, void* dw,
+                         void* db) {
+  using B = FlatBatch<T, G, R>;
+  constexpr int UPT = kFlatUpt;
+  constexpr uint32_t X0 = B::ROOM, S0 = X0 + (KEPT ? B::CODES : B::ROOM), STAGE = S0 + (KEPT ? B::SCALES : 0);
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ __align__(16) float ws[2][B::NT / 32 * 2 * R];
+  const int t = threadIdx.x % G, group = threadIdx.x / G;
+  auto count = [&](uint64_t r0) { return (uint32_t)min((uint64_t)B::ROWS, rows - r0); };
+  auto fetch = [&](uint64_t r0, uint8_t* at) {
+    FlatRun<T>(dy, (long long)r0 * C, count(r0) * C).fetch(at);
+    if constexpr (KEPT) {
+      FlatRun<int8_t>(k.codes, (long long)r0 * k.Cp, count(r0) * k.Cp).fetch(at + X0);
+      FlatRun<uint8_t>(k.scales, (long long)r0 * k.nbp, count(r0) * k.nbp).fetch(at + S0);
+    } else {
+      FlatRun<T>(x, (long long)r0 * C, count(r0) * C).fetch(at + X0);
+    }
+  };
+  const uint64_t step = (uint64_t)gridDim.x * B::ROWS;
+  uint64_t r0 = (uint64_t)blockIdx.x * B::ROWS;
+  constexpr int DEPTH = flat_depth(G);
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; ++d) {
+    if (r0 + d * step < rows) fetch(r0 + d * step, ring + d * STAGE);
+    copy_commit();
+  }
+  float w[UPT][4], aw[UPT * 4], ab[UPT * 4];
+  int n[UPT];
+#pragma unroll
+  for (int i = 0; i < UPT; ++i) {
+    const int c = (t + i * G) * 4;
+    n[i] = max(0, min(4, C - c));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[i][j] = j < n[i] ? vec_at(vec.w, vec.fp32, c + j, 1.f) : 0.f;
+      aw[i * 4 + j] = ab[i * 4 + j] = 0.f;
+    }
+  }
+  const float inv_c = 1.f / C;
+  int stage = 0, flip = 0;
+  for (; r0 < rows; r0 += step, stage = stage == DEPTH - 1 ? 0 : stage + 1, flip ^= 1) {
+    const uint64_t ahead = r0 + (DEPTH - 1) * step;
+    if (ahead < rows) fetch(ahead, ring + (stage == 0 ? DEPTH - 1 : stage - 1) * STAGE);
+    copy_commit();
+    copy_wait<DEPTH - 1>();
+    float2 st[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const uint64_t r = r0 + q * B::GROUPS + group;
+      st[q] = r < rows ? *reinterpret_cast<const float2*>(stats + 2 * r) : make_float2(0.f, 0.f);
+    }
+    __syncthreads();
+    uint8_t* at = ring + stage * STAGE;
+    const uint32_t head = FlatRun<T>(dy, (long long)r0 * C, 0).head;
+    T* gt = reinterpret_cast<T*>(at + head);
+    const T* xt = reinterpret_cast<const T*>(at + X0 + head);
+    const uint8_t* ct = at + X0;
+    const uint8_t* bt = at + S0 + (r0 * k.nbp & 15);
+    float gw[R][UPT][4], d[R][UPT][4], s[2 * R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const int row = q * B::GROUPS + group;
+      const bool in = r0 + row < rows;
+      s[2 * q] = s[2 * q + 1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        const int c = (t + i * G) * 4, m = in ? n[i] : 0;
+        float g[4];
+        read4(gt + row * C + c, m, g);
+        if constexpr (KEPT) {
+          const uint32_t u = m > 0 ? *reinterpret_cast<const uint32_t*>(ct + row * k.Cp + c) ^ 0x80808080u : 0x80808080u;
+          const float unit = m > 0 ? kept8_step(bt[row * k.nbp + c / kKeptBlock]) : 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            d[q][i][j] = fmaf(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + j)) - 8388736.f, unit, -st[q].x);
+        } else {
+          read4(xt + row * C + c, m, d[q][i]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d[q][i][j] -= st[q].x;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // past the row's end g is zero and d some finite number unless the row is not
+          const float gr = g[j] * st[q].y;
+          gw[q][i][j] = gr * w[i][j];
+          s[2 * q] = fmaf(gw[q][i][j], d[q][i][j], s[2 * q]);
+          s[2 * q + 1] += gw[q][i][j];
+          aw[i * 4 + j] = fmaf(gr, d[q][i][j], aw[i * 4 + j]);
+          ab[i * 4 + j] += g[j];
+        }
+      }
+    }
+    if (dx != nullptr) {
+      group_sum<G, 2 * R>(s, ws[flip]);
+#pragma unroll
+      for (int q = 0; q < R; ++q) {
+        const int row = q * B::GROUPS + group;
+        if (r0 + row >= rows) continue;
+        const float a = layer ? s[2 * q + 1] * inv_c : 0.f, b = -s[2 * q] * inv_c * st[q].y * st[q].y;
+#pragma unroll
+        for (int i = 0; i < UPT; ++i) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d[q][i][j] = fmaf(d[q][i][j], b, gw[q][i][j] - a);
+          write4(gt + row * C + (t + i * G) * 4, n[i], d[q][i]);
+        }
+      }
+      __syncthreads();
+      FlatRun<T>(dx, (long long)r0 * C, count(r0) * C).store(at);  // dx is aligned as dy is: the same offsets
+    }
+    __syncthreads();
+  }
+  if (part == nullptr) return;
+  join_groups<G, B::GROUPS>(aw, t, group);
+  join_groups<G, B::GROUPS>(ab, t, group);
+  if (group != 0) return;
+#pragma unroll
+  for (int i = 0; i < UPT; ++i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j >= n[i]) continue;
+      store_partial(aw[i * 4 + j], (t + i * G) * 4 + j, C, 0, vec.fp32, part, dw);
+      store_partial(ab[i * 4 + j], (t + i * G) * 4 + j, C, 1, vec.fp32, part, db);
+    }
+  }
+}
+
 // ---------------------------------------------------------------- single-column form
-// Rows that 16-byte copies cannot address (odd widths, odd offsets): thread t of a group of whole warps holds columns
-// t + i G, so a warp's 32 neighbouring columns are one block of the codes.
-constexpr int single_ctas(int G) { return threads_of(G) > 512 ? 1 : 768 / threads_of(G); }
+// Views that are neither (odd column slices, odd offsets), read where they lie: thread t of a group of whole warps holds
+// columns t + i G, so a warp's 32 neighbouring columns are one block of the codes.
+constexpr int single_ctas(int G) { return threads_of(G) <= 256 ? 2 : 1; }
 template <typename T, int G, int E, int R>
 __global__ void __launch_bounds__(threads_of(G), single_ctas(G))
     norm_fwd_single_kernel(RowView x, uint32_t rows, int C, Vectors vec, float eps, bool layer, T* __restrict__ y,
@@ -567,7 +828,7 @@ __global__ void __launch_bounds__(threads_of(G), single_ctas(G))
 }
 
 template <typename T, int G, int E, int R, bool KEPT>
-__global__ void __launch_bounds__(threads_of(G), 512 / threads_of(G) > 0 ? 512 / threads_of(G) : 1)
+__global__ void __launch_bounds__(threads_of(G), single_ctas(G))
     norm_bwd_single_kernel(RowView dy, RowView x, Kept k, uint32_t rows, int C, Vectors vec, bool layer,
                            const float* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, void* dw,
                            void* db) {
@@ -780,6 +1041,9 @@ bool rows_aligned16(const RowsArg& a, bool fp32) {
   return aligned16(a.p) && a.outer_stride * e % 16 == 0 && a.inner_stride * e % 16 == 0;
 }
 
+// Whether `a` is a contiguous, 16-byte aligned tensor of rows of C.
+bool contiguous_rows(const RowsArg& a, int C) { return a.inner == 1 && a.outer_stride == C && aligned16(a.p); }
+
 int sm_count() {
   static int n = 0;
   if (n == 0) {
@@ -828,6 +1092,19 @@ void fwd_single(const FwdCall& f) {
       view_of(f.x), (uint32_t)f.a.rows, f.a.C, f.vec(), f.a.eps, f.a.layer, (T*)f.y, f.stats, kept_of(f.k));
 }
 
+template <typename T, int G, int R>
+void fwd_flat(const FwdCall& f) {
+  using B = FlatBatch<T, G, R>;
+  constexpr int BYTES = flat_depth(G) * B::ROOM;
+  static_assert(BYTES * flat_ctas(G, R) <= kRingBudget, "the batches of an SM's CTAs do not fit its shared memory");
+  const auto kernel = norm_fwd_flat_kernel<T, G, R>;
+  static bool ready = false;
+  if (!ready) ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) == cudaSuccess;
+  kernel<<<grid_for(f.a.rows, B::ROWS, flat_ctas(G, R)), B::NT, BYTES, f.s>>>((const T*)f.x.p, (uint32_t)f.a.rows, f.a.C,
+                                                                           f.vec(), f.a.eps, f.a.layer, (T*)f.y,
+                                                                           f.stats, kept_of(f.k));
+}
+
 template <typename T, bool LAYER>
 void fwd_staged_any(const FwdCall& f) {
   const int C = f.a.C;
@@ -850,12 +1127,19 @@ void fwd(const FwdCall& f) {
   const int C = f.a.C;
   if (C % 8 == 0 && C <= 16384 && rows_aligned16(f.x, f.a.fp32) && aligned16(f.a.w) && aligned16(f.a.b))
     return f.a.layer ? fwd_staged_any<T, true>(f) : fwd_staged_any<T, false>(f);
-  if (C <= 256) return fwd_single<T, 32, 8, 4>(f);
-  if (C <= 1024) return fwd_single<T, 128, 8, 4>(f);
-  if (C <= 2048) return fwd_single<T, 256, 8, 4>(f);
-  if (C <= 4096) return fwd_single<T, 256, 16, 2>(f);
-  if (C <= 8192) return fwd_single<T, 512, 16, 2>(f);
-  if (C <= 16384) return fwd_single<T, 1024, 16, 1>(f);
+  // batches of about 8 KB
+  constexpr int R = sizeof(T) == 2 ? 2 : 1;
+  if (contiguous_rows(f.x, C)) {
+    if (C <= 256) return fwd_flat<T, 32, R>(f);
+    if (C <= 512) return fwd_flat<T, 64, R>(f);
+    if (C <= 1024) return fwd_flat<T, 128, R>(f);
+    if (C <= 2048) return fwd_flat<T, 256, R>(f);
+    if (C <= 4096) return fwd_flat<T, 512, R>(f);
+    if (C <= 8192) return fwd_flat<T, 1024, 1>(f);
+  }
+  if (C <= 256) return fwd_single<T, 32, 8, 2>(f);
+  if (C <= 2048) return fwd_single<T, 256, 8, 2>(f);
+  if (C <= 8192) return fwd_single<T, 512, 16, 1>(f);
   norm_fwd_wide_kernel<T><<<wide_grid(f.a.rows), kThreads, 0, f.s>>>(view_of(f.x), (uint32_t)f.a.rows, C, f.vec(),
                                                                      f.a.eps, f.a.layer, (T*)f.y, f.stats,
                                                                      kept_of(f.k));
@@ -900,7 +1184,7 @@ void bwd_staged(const BwdCall& b) {
 template <typename T, int G, int E, int R, bool KEPT>
 void bwd_single(const BwdCall& b) {
   constexpr int NT = threads_of(G), GROUPS = NT / G;
-  const int grid = grid_for(b.a.rows, GROUPS * R, 512 / NT > 0 ? 512 / NT : 1);
+  const int grid = grid_for(b.a.rows, GROUPS * R, single_ctas(G));
   if (b.parts != nullptr) {
     *b.parts = grid;
     return;
@@ -908,6 +1192,24 @@ void bwd_single(const BwdCall& b) {
   norm_bwd_single_kernel<T, G, E, R, KEPT><<<grid, NT, 0, b.s>>>(view_of(b.dy), view_of(b.x), kept_of(b.k),
                                                                  (uint32_t)b.a.rows, b.a.C, b.vec(), b.a.layer,
                                                                  b.stats, (T*)b.dx, b.part, b.dw, b.db);
+  b.finish(grid);
+}
+
+template <typename T, int G, int R, bool KEPT>
+void bwd_flat(const BwdCall& b) {
+  using B = FlatBatch<T, G, R>;
+  constexpr int BYTES = flat_depth(G) * (B::ROOM + (KEPT ? B::CODES + B::SCALES : B::ROOM));
+  static_assert(BYTES * flat_ctas(G, R) <= kRingBudget, "the batches of an SM's CTAs do not fit its shared memory");
+  const int grid = grid_for(b.a.rows, B::ROWS, flat_ctas(G, R));
+  if (b.parts != nullptr) {
+    *b.parts = grid;
+    return;
+  }
+  const auto kernel = norm_bwd_flat_kernel<T, G, R, KEPT>;
+  static bool ready = false;
+  if (!ready) ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) == cudaSuccess;
+  kernel<<<grid, B::NT, BYTES, b.s>>>((const T*)b.dy.p, (const T*)b.x.p, kept_of(b.k), (uint32_t)b.a.rows, b.a.C,
+                                      b.vec(), b.a.layer, b.stats, (T*)b.dx, b.part, b.dw, b.db);
   b.finish(grid);
 }
 
@@ -953,10 +1255,17 @@ void bwd(const BwdCall& b) {
   const bool fp32 = sizeof(T) == 4;
   if (C % 8 == 0 && C <= 16384 && rows_aligned16(b.dy, fp32) && (KEPT || rows_aligned16(b.x, fp32)) && aligned16(b.a.w))
     return b.a.layer ? bwd_staged_any<T, true, KEPT>(b) : bwd_staged_any<T, false, KEPT>(b);
+  constexpr int R = sizeof(T) == 2 ? 2 : 1;
+  if (contiguous_rows(b.dy, C) && (KEPT || contiguous_rows(b.x, C))) {
+    if (C <= 256) return bwd_flat<T, 32, R, KEPT>(b);
+    if (C <= 512) return bwd_flat<T, 64, R, KEPT>(b);
+    if (C <= 1024) return bwd_flat<T, 128, R, KEPT>(b);
+    if (C <= 2048) return bwd_flat<T, 256, R, KEPT>(b);
+    if (C <= 4096) return bwd_flat<T, 512, R, KEPT>(b);
+    if (C <= 8192) return bwd_flat<T, 1024, 1, KEPT>(b);
+  }
   if (C <= 256) return bwd_single<T, 32, 8, 2, KEPT>(b);
-  if (C <= 1024) return bwd_single<T, 128, 8, 2, KEPT>(b);
   if (C <= 2048) return bwd_single<T, 256, 8, 2, KEPT>(b);
-  if (C <= 4096) return bwd_single<T, 512, 8, 1, KEPT>(b);
   if (C <= 8192) return bwd_single<T, 1024, 8, 1, KEPT>(b);
   bwd_wide<T>(b);
 }

@@ -37,6 +37,19 @@ def test_store_equals_the_definition(rows, C, dtype):
 
 
 @DTYPES
+@pytest.mark.parametrize("rows,C", [(3000, 7), (1, 4099), (257, 4097), (40, 12305), (1000, 2047), (2, 8191), (5000, 129)])
+def test_store_odd_widths(rows, C, dtype):
+    x = acts(rows, C, dtype=dtype, seed=C)
+    x[rows // 2, C // 2] = float("nan")
+    got, want = restore8(keep8(x)).cpu().double(), R.kept_values(x)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+    cpu = keep8(x[:rows // 2].cpu())
+    kept = keep8(x)
+    assert torch.equal(cpu.codes, kept.codes[:rows // 2].cpu()) and torch.equal(cpu.scales, kept.scales[:rows // 2].cpu())
+
+
+@DTYPES
 def test_store_of_special_values(dtype):
     x = torch.zeros(7, 72, device="cuda", dtype=dtype)
     x[1, 3], x[2, 40], x[2, 41] = float("inf"), float("nan"), float("-inf")
@@ -156,6 +169,14 @@ def test_norm_of_narrow_rows(C, dtype, layer, kept):
 
 @DTYPES
 @KEPT
+@pytest.mark.parametrize("rows,C", [(20011, 33), (1, 257), (9000, 511), (1300, 1023), (700, 2047), (301, 3001), (611, 4097),
+                                    (150, 8191), (12, 8193)])
+def test_norm_odd_widths(rows, C, dtype, kept):
+    norm_case((rows, C), dtype, True, kept, seed=C)
+
+
+@DTYPES
+@KEPT
 def test_norm_long(dtype, kept):
     norm_case((30011, 264), dtype, True, kept)
 
@@ -249,7 +270,8 @@ def test_norm_gradient_against_differences():
 
 # ------------------------------------------------------------------------------------ SwiGLU
 @DTYPES
-@pytest.mark.parametrize("rows,C", [(1, 1), (1, 16384), (300, 40), (77, 1001), (5, 33), (0, 64), (1025, 512)])
+@pytest.mark.parametrize("rows,C", [(1, 1), (1, 16384), (300, 40), (77, 1001), (5, 33), (0, 64), (1025, 512), (37, 4099),
+                                    (2000, 65)])
 def test_swiglu(rows, C, dtype):
     gate = acts(rows, C, dtype=dtype).requires_grad_(True)
     value = acts(rows, C, dtype=dtype, seed=1).requires_grad_(True)
