@@ -502,14 +502,15 @@ __global__ void __launch_bounds__(threads_of(G), CTAS)
 // ahead left the kernel waiting for memory at 35 % of its bandwidth).  Fragment i of thread t are the 4 columns from 4 (t + i G) on: eight lanes hold a block of
 // the codes.  Results take the place of the input and leave as one run.
 constexpr int flat_ctas(int G, int R) { return threads_of(G) > 256 ? 1 : R == 1 ? 3 : 2; }
-constexpr int flat_depth(int G) { return threads_of(G) <= 512 ? 4 : 3; }
+constexpr int flat_depth(int G) { return 3; }
 constexpr int kFlatUpt = 2;
 
 template <typename T, int G, int R>
 struct FlatBatch {
   static constexpr int NT = threads_of(G), GROUPS = NT / G, ROWS = GROUPS * R, WIDTH = G * kFlatUpt * 4;
   static constexpr uint32_t ROOM = FlatRun<T>::room(ROWS * WIDTH);
-  static constexpr uint32_t CODES = FlatRun<int8_t>::room(ROWS * WIDTH), SCALES = FlatRun<uint8_t>::room(ROWS * (WIDTH / kKeptBlock));
+  static constexpr uint32_t CODES = FlatRun<int8_t>::room(ROWS * WIDTH);
+  static constexpr uint32_t SCALES = FlatRun<uint8_t>::room(ROWS * ((WIDTH / kKeptBlock + 3) / 4 * 4));
 };
 
 // `n` of the four elements from p on, zeros for the others.
@@ -596,20 +597,20 @@ __global__ void __launch_bounds__(threads_of(G), flat_ctas(G, R))
     for (int q = 0; q < R; ++q) {
       const int row = q * B::GROUPS + group;
       const uint64_t r = r0 + row;
-      if (r >= rows) continue;  // the whole group
+      const bool in = r < rows;
       const float rstd = rsqrtf(var[q] * inv_c + eps);
-      if (t == 0 && stats != nullptr) *reinterpret_cast<float2*>(stats + 2 * r) = make_float2(mean[q], rstd);
+      if (in && t == 0 && stats != nullptr) *reinterpret_cast<float2*>(stats + 2 * r) = make_float2(mean[q], rstd);
 #pragma unroll
       for (int i = 0; i < UPT; ++i) {
         const int c = (t + i * G) * 4;
-        if (k.codes != nullptr) {
+        if (k.codes != nullptr) {  // all lanes
           uint32_t m = 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(v[q][i][j]) & 0x7fffffffu);
 #pragma unroll
           for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
           const uint32_t sb = kept8_byte(m);
-          if (c < k.Cp) {
+          if (in && c < k.Cp) {
             const float inv = kept8_inv_step(sb);
             *reinterpret_cast<uint32_t*>(k.codes + (long long)r * k.Cp + c) =
                 pack4_low_bytes(kept8_code(v[q][i][0], inv), kept8_code(v[q][i][1], inv), kept8_code(v[q][i][2], inv),
@@ -619,7 +620,7 @@ __global__ void __launch_bounds__(threads_of(G), flat_ctas(G, R))
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[q][i][j] = fmaf((v[q][i][j] - mean[q]) * rstd, w[i][j], b[i][j]);
-        write4(tile + row * C + c, n[i], v[q][i]);
+        write4(tile + row * C + c, in ? n[i] : 0, v[q][i]);
       }
     }
     __syncthreads();
@@ -1127,14 +1128,16 @@ void fwd(const FwdCall& f) {
   const int C = f.a.C;
   if (C % 8 == 0 && C <= 16384 && rows_aligned16(f.x, f.a.fp32) && aligned16(f.a.w) && aligned16(f.a.b))
     return f.a.layer ? fwd_staged_any<T, true>(f) : fwd_staged_any<T, false>(f);
-  // batches of about 8 KB
-  constexpr int R = sizeof(T) == 2 ? 2 : 1;
+  // batches of about 16 KB
+  constexpr int R = sizeof(T) == 2 ? 4 : 2;
   if (contiguous_rows(f.x, C)) {
+    if (C <= 64) return fwd_flat<T, 8, R>(f);
+    if (C <= 128) return fwd_flat<T, 16, R>(f);
     if (C <= 256) return fwd_flat<T, 32, R>(f);
     if (C <= 512) return fwd_flat<T, 64, R>(f);
     if (C <= 1024) return fwd_flat<T, 128, R>(f);
     if (C <= 2048) return fwd_flat<T, 256, R>(f);
-    if (C <= 4096) return fwd_flat<T, 512, R>(f);
+    if (C <= 4096) return fwd_flat<T, 512, 2>(f);
     if (C <= 8192) return fwd_flat<T, 1024, 1>(f);
   }
   if (C <= 256) return fwd_single<T, 32, 8, 2>(f);
@@ -1255,8 +1258,10 @@ void bwd(const BwdCall& b) {
   const bool fp32 = sizeof(T) == 4;
   if (C % 8 == 0 && C <= 16384 && rows_aligned16(b.dy, fp32) && (KEPT || rows_aligned16(b.x, fp32)) && aligned16(b.a.w))
     return b.a.layer ? bwd_staged_any<T, true, KEPT>(b) : bwd_staged_any<T, false, KEPT>(b);
-  constexpr int R = sizeof(T) == 2 ? 2 : 1;
+  constexpr int R = 2;
   if (contiguous_rows(b.dy, C) && (KEPT || contiguous_rows(b.x, C))) {
+    if (C <= 64) return bwd_flat<T, 8, R, KEPT>(b);
+    if (C <= 128) return bwd_flat<T, 16, R, KEPT>(b);
     if (C <= 256) return bwd_flat<T, 32, R, KEPT>(b);
     if (C <= 512) return bwd_flat<T, 64, R, KEPT>(b);
     if (C <= 1024) return bwd_flat<T, 128, R, KEPT>(b);
