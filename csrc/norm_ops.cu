@@ -503,11 +503,10 @@ __global__ void __launch_bounds__(threads_of(G), CTAS)
 // the codes.  Results take the place of the input and leave as one run.
 constexpr int flat_ctas(int G, int R) { return threads_of(G) > 256 ? 1 : R == 1 ? 3 : 2; }
 constexpr int flat_depth(int G) { return 3; }
-constexpr int kFlatUpt = 2;
 
-template <typename T, int G, int R>
+template <typename T, int G, int UPT, int R>
 struct FlatBatch {
-  static constexpr int NT = threads_of(G), GROUPS = NT / G, ROWS = GROUPS * R, WIDTH = G * kFlatUpt * 4;
+  static constexpr int NT = threads_of(G), GROUPS = NT / G, ROWS = GROUPS * R, WIDTH = G * UPT * 4;
   static constexpr uint32_t ROOM = FlatRun<T>::room(ROWS * WIDTH);
   static constexpr uint32_t CODES = FlatRun<int8_t>::room(ROWS * WIDTH);
   static constexpr uint32_t SCALES = FlatRun<uint8_t>::room(ROWS * ((WIDTH / kKeptBlock + 3) / 4 * 4));
@@ -526,12 +525,11 @@ __device__ __forceinline__ void write4(T* p, int n, const float (&v)[4]) {
     if (j < n) p[j] = from_f32<T>(v[j]);
 }
 
-template <typename T, int G, int R>
+template <typename T, int G, int UPT, int R>
 __global__ void __launch_bounds__(threads_of(G), flat_ctas(G, R))
     norm_fwd_flat_kernel(const T* x, uint32_t rows, int C, Vectors vec, float eps, bool layer, T* __restrict__ y,
                          float* __restrict__ stats, Kept k) {
-  using B = FlatBatch<T, G, R>;
-  constexpr int UPT = kFlatUpt;
+  using B = FlatBatch<T, G, UPT, R>;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ __align__(16) float ws[2][2][B::NT / 32 * R];
   const int t = threadIdx.x % G, group = threadIdx.x / G;
@@ -629,13 +627,12 @@ __global__ void __launch_bounds__(threads_of(G), flat_ctas(G, R))
   }
 }
 
-template <typename T, int G, int R, bool KEPT>
+template <typename T, int G, int UPT, int R, bool KEPT>
 __global__ void __launch_bounds__(threads_of(G), flat_ctas(G, R))
     norm_bwd_flat_kernel(const T* dy, const T* x, Kept k, uint32_t rows, int C, Vectors vec, bool layer,
                          const float* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, void* dw,
                          void* db) {
-  using B = FlatBatch<T, G, R>;
-  constexpr int UPT = kFlatUpt;
+  using B = FlatBatch<T, G, UPT, R>;
   constexpr uint32_t X0 = B::ROOM, S0 = X0 + (KEPT ? B::CODES : B::ROOM), STAGE = S0 + (KEPT ? B::SCALES : 0);
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ __align__(16) float ws[2][B::NT / 32 * 2 * R];
@@ -1093,12 +1090,12 @@ void fwd_single(const FwdCall& f) {
       view_of(f.x), (uint32_t)f.a.rows, f.a.C, f.vec(), f.a.eps, f.a.layer, (T*)f.y, f.stats, kept_of(f.k));
 }
 
-template <typename T, int G, int R>
+template <typename T, int G, int UPT, int R>
 void fwd_flat(const FwdCall& f) {
-  using B = FlatBatch<T, G, R>;
+  using B = FlatBatch<T, G, UPT, R>;
   constexpr int BYTES = flat_depth(G) * B::ROOM;
   static_assert(BYTES * flat_ctas(G, R) <= kRingBudget, "the batches of an SM's CTAs do not fit its shared memory");
-  const auto kernel = norm_fwd_flat_kernel<T, G, R>;
+  const auto kernel = norm_fwd_flat_kernel<T, G, UPT, R>;
   static bool ready = false;
   if (!ready) ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) == cudaSuccess;
   kernel<<<grid_for(f.a.rows, B::ROWS, flat_ctas(G, R)), B::NT, BYTES, f.s>>>((const T*)f.x.p, (uint32_t)f.a.rows, f.a.C,
@@ -1131,14 +1128,14 @@ void fwd(const FwdCall& f) {
   // batches of about 16 KB
   constexpr int R = sizeof(T) == 2 ? 4 : 2;
   if (contiguous_rows(f.x, C)) {
-    if (C <= 64) return fwd_flat<T, 8, R>(f);
-    if (C <= 128) return fwd_flat<T, 16, R>(f);
-    if (C <= 256) return fwd_flat<T, 32, R>(f);
-    if (C <= 512) return fwd_flat<T, 64, R>(f);
-    if (C <= 1024) return fwd_flat<T, 128, R>(f);
-    if (C <= 2048) return fwd_flat<T, 256, R>(f);
-    if (C <= 4096) return fwd_flat<T, 512, 2>(f);
-    if (C <= 8192) return fwd_flat<T, 1024, 1>(f);
+    if (C <= 64) return fwd_flat<T, 8, 2, R>(f);
+    if (C <= 128) return fwd_flat<T, 16, 2, R>(f);
+    if (C <= 256) return fwd_flat<T, 32, 2, R>(f);
+    if (C <= 512) return fwd_flat<T, 64, 2, R>(f);
+    if (C <= 1024) return fwd_flat<T, 128, 2, R>(f);
+    if (C <= 2048) return fwd_flat<T, 256, 2, R>(f);
+    if (C <= 4096) return fwd_flat<T, 512, 2, 2>(f);
+    if (C <= 8192) return fwd_flat<T, 512, 4, sizeof(T) == 2 ? 2 : 1>(f);
   }
   if (C <= 256) return fwd_single<T, 32, 8, 2>(f);
   if (C <= 2048) return fwd_single<T, 256, 8, 2>(f);
@@ -1198,9 +1195,9 @@ void bwd_single(const BwdCall& b) {
   b.finish(grid);
 }
 
-template <typename T, int G, int R, bool KEPT>
+template <typename T, int G, int UPT, int R, bool KEPT>
 void bwd_flat(const BwdCall& b) {
-  using B = FlatBatch<T, G, R>;
+  using B = FlatBatch<T, G, UPT, R>;
   constexpr int BYTES = flat_depth(G) * (B::ROOM + (KEPT ? B::CODES + B::SCALES : B::ROOM));
   static_assert(BYTES * flat_ctas(G, R) <= kRingBudget, "the batches of an SM's CTAs do not fit its shared memory");
   const int grid = grid_for(b.a.rows, B::ROWS, flat_ctas(G, R));
@@ -1208,7 +1205,7 @@ void bwd_flat(const BwdCall& b) {
     *b.parts = grid;
     return;
   }
-  const auto kernel = norm_bwd_flat_kernel<T, G, R, KEPT>;
+  const auto kernel = norm_bwd_flat_kernel<T, G, UPT, R, KEPT>;
   static bool ready = false;
   if (!ready) ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) == cudaSuccess;
   kernel<<<grid, B::NT, BYTES, b.s>>>((const T*)b.dy.p, (const T*)b.x.p, kept_of(b.k), (uint32_t)b.a.rows, b.a.C,
@@ -1260,14 +1257,14 @@ void bwd(const BwdCall& b) {
     return b.a.layer ? bwd_staged_any<T, true, KEPT>(b) : bwd_staged_any<T, false, KEPT>(b);
   constexpr int R = 2;
   if (contiguous_rows(b.dy, C) && (KEPT || contiguous_rows(b.x, C))) {
-    if (C <= 64) return bwd_flat<T, 8, R, KEPT>(b);
-    if (C <= 128) return bwd_flat<T, 16, R, KEPT>(b);
-    if (C <= 256) return bwd_flat<T, 32, R, KEPT>(b);
-    if (C <= 512) return bwd_flat<T, 64, R, KEPT>(b);
-    if (C <= 1024) return bwd_flat<T, 128, R, KEPT>(b);
-    if (C <= 2048) return bwd_flat<T, 256, R, KEPT>(b);
-    if (C <= 4096) return bwd_flat<T, 512, R, KEPT>(b);
-    if (C <= 8192) return bwd_flat<T, 1024, 1, KEPT>(b);
+    if (C <= 64) return bwd_flat<T, 8, 2, R, KEPT>(b);
+    if (C <= 128) return bwd_flat<T, 16, 2, R, KEPT>(b);
+    if (C <= 256) return bwd_flat<T, 32, 2, R, KEPT>(b);
+    if (C <= 512) return bwd_flat<T, 64, 2, R, KEPT>(b);
+    if (C <= 1024) return bwd_flat<T, 128, 2, R, KEPT>(b);
+    if (C <= 2048) return bwd_flat<T, 256, 2, R, KEPT>(b);
+    if (C <= 4096) return bwd_flat<T, 512, 2, R, KEPT>(b);
+    if (C <= 8192) return bwd_flat<T, 512, 4, 1, KEPT>(b);
   }
   if (C <= 256) return bwd_single<T, 32, 8, 2, KEPT>(b);
   if (C <= 2048) return bwd_single<T, 256, 8, 2, KEPT>(b);
