@@ -680,7 +680,7 @@ void ns_scale_by_invnorm(torch::Tensor Q, torch::Tensor norm2, double eps) {
 
 int error_flag(bool reset) {
   return gemm_error_flag(reset) | packed_ops_error_flag(reset) | attn_error_flag(reset) | comm_error_flag(reset) |
-         qkv_bounds_error(reset);
+         qkv_bounds_error(reset) | wgrad_error_flag(reset);
 }
 
 // ---------------------------------------------------------------- peer-memory collectives

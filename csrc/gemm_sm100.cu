@@ -23,6 +23,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "gemm_host.h"
 #include "launchers.h"
 #include "sm100.cuh"
 

@@ -301,7 +301,7 @@ torch::Tensor weight_operand(const torch::Tensor& w_) {
 }
 
 // rows of the kept input reloaded at a time for a weight gradient (bounds the bf16 temporary)
-constexpr int64_t kWgradRows = 16384;
+constexpr int64_t kWgradRows = 32768;
 
 // dW [N, K] = g [rows, N]^T x, x the kept [rows, K] matrix, in fp32 or bf16.  `gp` is g as an operand.
 torch::Tensor weight_grad8(const torch::Tensor& gp, int64_t N, const torch::Tensor& codes, const torch::Tensor& scales,
@@ -310,17 +310,23 @@ torch::Tensor weight_grad8(const torch::Tensor& gp, int64_t N, const torch::Tens
   const auto dt = fp32 ? torch::kFloat32 : torch::kBFloat16;
   if (rows == 0) return torch::zeros({N, K}, gp.options().dtype(dt));
   const Kept8Buf k = kept_of(codes, scales, rows, K);
-  const bool one = rows <= kWgradRows;
-  auto out = torch::empty({up8(N), up8(K)}, gp.options().dtype(one ? dt : torch::kFloat32));
+  const bool one = rows <= kWgradRows;  // later chunks add to fp32
   auto x = torch::empty({one ? rows : kWgradRows, up8(K)}, gp.options());
+  auto dw = torch::empty({N, up8(K)}, gp.options().dtype(one ? dt : torch::kFloat32));
   for (int64_t r0 = 0; r0 < rows; r0 += kWgradRows) {
     const int64_t n = std::min(kWgradRows, rows - r0);
     launch_restore8(k, r0, n, false, x.data_ptr(), x.size(1), (int)x.size(1), stream());
-    gemm(gp.narrow(0, r0, n), x.narrow(0, 0, n), out, false, false, c10::nullopt, c10::nullopt, r0 > 0);
+    const WgradPlan plan = wgrad_plan(n, (int)N, (int)K);
+    torch::Tensor part;
+    if (plan.part_floats > 0) part = torch::empty({plan.part_floats}, gp.options().dtype(torch::kFloat32));
+    check_launch(launch_wgrad(plan, static_cast<const char*>(gp.data_ptr()) + 2 * r0 * gp.stride(0), gp.stride(0),
+                              x.data_ptr(), x.size(1), n, (int)N, (int)K, dw.data_ptr(), dw.size(1),
+                              dw.scalar_type() == torch::kFloat32, r0 > 0,
+                              part.defined() ? part.data_ptr<float>() : nullptr, stream()),
+                 "weight_grad8");
   }
-  check_launch(nullptr, "weight_grad8");
-  auto dw = out.narrow(0, 0, N).narrow(1, 0, K);
-  return dw.scalar_type() == dt ? dw : dw.to(dt);
+  if (dw.scalar_type() != dt) dw = dw.to(dt);
+  return K % 8 == 0 ? dw : dw.narrow(1, 0, K);
 }
 
 struct LinearNode : torch::autograd::Function<LinearNode> {

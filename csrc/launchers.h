@@ -76,6 +76,19 @@ int norm_bwd_parts(const NormArgs& a, const RowsArg& dy, const RowsArg& x, const
 void launch_norm_bwd(const NormArgs& a, const RowsArg& dy, const RowsArg& x, const Kept8Buf& k, const float* stats,
                      void* dx, float* part, void* dw, void* db, cudaStream_t s);
 
+// ------------------------------------------------------------------ wgrad_sm100.cu
+// dW [n, k] (+)= dY [rows, n]^T X [rows, k]; tiles that are split over the rows need scratch.
+struct WgradPlan {
+  int whole, split, pieces;
+  long long part_floats;
+};
+WgradPlan wgrad_plan(long long rows, int n, int k);
+// dy, x: bf16, row strides multiples of 8; d: bf16 or fp32 with row stride ldd >= k rounded up to 8; add: fp32 only.
+const char* launch_wgrad(const WgradPlan& plan, const void* dy, long long lddy, const void* x, long long ldx,
+                         long long rows, int n, int k, void* d, long long ldd, bool d_fp32, bool add, float* part,
+                         cudaStream_t s);
+int wgrad_error_flag(bool reset);
+
 // ------------------------------------------------------------------ gemm_sm100.cu
 constexpr int kGemmMaxGroups = 4;
 struct GemmGroup {
