@@ -1,7 +1,7 @@
 // Python bindings of the 8-bit kept activations and the norms: tensor validation, output allocation, and the
-// autograd nodes.  The nodes are C++ (the other ops' are Python): these operators also run on a few rows,
-// where a Python node's host time is most of a forward and backward (91 us of host time against 45 us
-// for a layer norm of one row; see the figures at NormNode).
+// autograd nodes.  The nodes are C++ where the other ops' are Python: these operators also run on a few rows, where
+// the host's time is the pass.  Of a layer norm's forward and backward of one row, 61 us on the host, the autograd engine takes 37;
+// a Python node added about 10.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -20,6 +20,16 @@ using OptTensor = c10::optional<torch::Tensor>;
 namespace {
 
 cudaStream_t stream() { return at::cuda::getCurrentCUDAStream(); }
+
+// Texts of error messages.  Built from strings alone: streaming a number from this file crashes with this image's pair
+// of compiler and C++ runtime.
+std::string shape_text(const torch::Tensor& t) {
+  std::string s = "(";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+  return s + ")";
+}
+std::string type_text(const torch::Tensor& t) { return c10::toString(t.scalar_type()); }
+std::string device_text(const torch::Tensor& t) { return t.device().str(); }
 
 void check_launch(const char* err, const char* what) {
   TORCH_CHECK(err == nullptr, what, ": ", err ? err : "");
@@ -42,9 +52,10 @@ struct RowsOf {
 };
 
 RowsOf rows_of(torch::Tensor t, const char* name) {
-  TORCH_CHECK(t.is_cuda() && (t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat32), name,
-              " must be a bf16 or fp32 CUDA tensor");
-  TORCH_CHECK(t.dim() >= 1 && t.size(-1) >= 1 && t.size(-1) < (1 << 30), name, " needs a last dimension of 1 .. 2^30");
+  TORCH_CHECK_TYPE(t.is_cuda() && (t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat32), name,
+                   " must be bf16 or fp32 on CUDA, got ", type_text(t));
+  TORCH_CHECK_VALUE(t.dim() >= 1 && t.size(-1) >= 1 && t.size(-1) < (1 << 30), name,
+                    " needs a last dimension of at least 1, got shape ", shape_text(t));
   if (t.size(-1) > 1 && t.stride(-1) != 1) t = t.contiguous();
   RowsOf r;
   r.C = (int)t.size(-1);
@@ -103,8 +114,9 @@ Kept8Buf kept_of(const torch::Tensor& codes, const torch::Tensor& scales, int64_
 }
 
 void check_same(const RowsOf& a, const RowsOf& b, const char* what) {
-  TORCH_CHECK(a.rows == b.rows && a.C == b.C && a.fp32 == b.fp32 && a.t.device() == b.t.device(), what,
-              ": shapes, dtypes or devices differ");
+  TORCH_CHECK_VALUE(a.rows == b.rows && a.C == b.C && a.fp32 == b.fp32 && a.t.device() == b.t.device(), what,
+                    " differ: ", shape_text(a.t), " ", type_text(a.t), " ", device_text(a.t), " and ", shape_text(b.t), " ",
+                    type_text(b.t), " ", device_text(b.t));
 }
 
 NormArgs norm_args(const RowsOf& x, const OptTensor& w, const OptTensor& b,
@@ -116,19 +128,24 @@ NormArgs norm_args(const RowsOf& x, const OptTensor& w, const OptTensor& b,
   a.layer = layer;
   a.eps = (float)eps;
   a.w_fp32 = x.fp32;
+  TORCH_CHECK_VALUE(eps >= 0, "eps=", std::to_string(eps), " is negative");
   const OptTensor* vs[2] = {&w, &b};
   const void** ps[2] = {&a.w, &a.b};
+  const char* names[2] = {"weight", "bias"};
   for (int i = 0; i < 2; ++i) {
     if (!vs[i]->has_value()) continue;
     const torch::Tensor& v = vs[i]->value();
-    TORCH_CHECK(v.dim() == 1 && v.size(0) == x.C && v.is_contiguous() && v.device() == x.t.device() &&
-                    (v.scalar_type() == torch::kFloat32 || v.scalar_type() == torch::kBFloat16),
-                "norm weight and bias must be contiguous bf16 or fp32 [C] tensors on x's device");
+    TORCH_CHECK_VALUE(v.dim() == 1 && v.size(0) == x.C, names[i], " ", shape_text(v),
+                      " does not fit rows of width ", std::to_string(x.C));
+    TORCH_CHECK_VALUE(v.device() == x.t.device(), names[i], " is on ", device_text(v), ", x on ", device_text(x.t));
+    TORCH_CHECK_TYPE(v.scalar_type() == torch::kFloat32 || v.scalar_type() == torch::kBFloat16, names[i],
+                     " must be bf16 or fp32, got ", type_text(v));
+    TORCH_CHECK(v.is_contiguous(), names[i], " must be contiguous");
     a.w_fp32 = v.scalar_type() == torch::kFloat32;
     *ps[i] = v.data_ptr();
   }
-  TORCH_CHECK(!w.has_value() || !b.has_value() || w->scalar_type() == b->scalar_type(),
-              "norm weight and bias must have one dtype");
+  TORCH_CHECK_TYPE(!w.has_value() || !b.has_value() || w->scalar_type() == b->scalar_type(),
+                   "weight and bias have different dtypes");
   return a;
 }
 
@@ -157,6 +174,18 @@ void restore8(torch::Tensor codes, torch::Tensor scales, int64_t C, int64_t row0
   launch_restore8(k, row0, out.size(0), out.scalar_type() == torch::kFloat32, out.data_ptr(), out.stride(0), (int)C,
                   stream());
   check_launch(nullptr, "restore8");
+}
+
+// The whole kept tensor in a new one of `shape`.
+torch::Tensor restore8_new(torch::Tensor codes, torch::Tensor scales, std::vector<int64_t> shape, bool fp32) {
+  const at::cuda::CUDAGuard guard(codes.device());
+  const int64_t C = shape.back();
+  const Kept8Buf k = kept_of(codes, scales, codes.size(0), C);
+  auto out = torch::empty(shape, codes.options().dtype(fp32 ? torch::kFloat32 : torch::kBFloat16));
+  TORCH_CHECK(out.numel() == codes.size(0) * C && codes.size(0) < (1ll << 31), "restore8: the shape has other rows");
+  launch_restore8(k, 0, codes.size(0), fp32, out.data_ptr(), C, (int)C, stream());
+  check_launch(nullptr, "restore8");
+  return out;
 }
 
 // (h, codes and scales of gate, codes and scales of value); without `keep` those are undefined
@@ -222,9 +251,8 @@ struct NormNode : torch::autograd::Function<NormNode> {
     if (grad) {
       ctx->save_for_backward({codes.defined() ? torch::Tensor() : x_, codes, scales, stats,
                               w.has_value() ? *w : torch::Tensor()});
-      ctx->saved_data["layer"] = layer;
-      ctx->saved_data["w_fp32"] = a.w_fp32;
-      ctx->saved_data["vectors"] = (int64_t)((w.has_value() ? 1 : 0) + (b.has_value() ? 2 : 0));
+      ctx->saved_data["flags"] =
+          (int64_t)((w.has_value() ? 1 : 0) + (b.has_value() ? 2 : 0) + (layer ? 4 : 0) + (a.w_fp32 ? 8 : 0));
     }
     return y;
   }
@@ -232,11 +260,10 @@ struct NormNode : torch::autograd::Function<NormNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const torch::Tensor& dy_ = grads[0];
     const variable_list saved = ctx->get_saved_variables();
-    const bool layer = ctx->saved_data["layer"].toBool(), w_fp32 = ctx->saved_data["w_fp32"].toBool();
-    const int64_t vectors = ctx->saved_data["vectors"].toInt();
-    const int w_edge = 1, b_edge = vectors & 1 ? 2 : 1;  // missing vectors have no edge
-    const bool need_dx = ctx->needs_input_grad(0), need_dw = (vectors & 1) && ctx->needs_input_grad(w_edge),
-               need_db = (vectors & 2) && ctx->needs_input_grad(b_edge);
+    const int64_t flags = ctx->saved_data["flags"].toInt();
+    const bool layer = flags & 4, w_fp32 = flags & 8;
+    const bool need_dx = ctx->needs_input_grad(0), need_dw = (flags & 1) && ctx->needs_input_grad(1),
+               need_db = (flags & 2) && ctx->needs_input_grad(flags & 1 ? 2 : 1);  // missing vectors have no edge
     const at::cuda::CUDAGuard guard(dy_.device());
     const RowsOf dy = rows_of(dy_, "dy");
     const torch::Tensor &codes = saved[1], &scales = saved[2], &stats = saved[3], &w = saved[4];
@@ -300,6 +327,19 @@ torch::Tensor weight_operand(const torch::Tensor& w_) {
   return out;
 }
 
+// dw (+)= g[row0 : row0 + rows]^T x[: rows]; g and x as operands.
+void run_wgrad(const torch::Tensor& gp, int64_t N, int64_t row0, const torch::Tensor& x, int64_t K, int64_t rows,
+               torch::Tensor& dw, bool add) {
+  const WgradPlan plan = wgrad_plan(rows, (int)N, (int)K);
+  torch::Tensor part;
+  if (plan.part_floats > 0) part = torch::empty({plan.part_floats}, gp.options().dtype(torch::kFloat32));
+  check_launch(launch_wgrad(plan, static_cast<const char*>(gp.data_ptr()) + 2 * row0 * gp.stride(0), gp.stride(0),
+                            x.data_ptr(), x.stride(0), rows, (int)N, (int)K, dw.data_ptr(), dw.size(1),
+                            dw.scalar_type() == torch::kFloat32, add,
+                            part.defined() ? part.data_ptr<float>() : nullptr, stream()),
+               "weight gradient");
+}
+
 // rows of the kept input reloaded at a time for a weight gradient (bounds the bf16 temporary)
 constexpr int64_t kWgradRows = 32768;
 
@@ -316,14 +356,7 @@ torch::Tensor weight_grad8(const torch::Tensor& gp, int64_t N, const torch::Tens
   for (int64_t r0 = 0; r0 < rows; r0 += kWgradRows) {
     const int64_t n = std::min(kWgradRows, rows - r0);
     launch_restore8(k, r0, n, false, x.data_ptr(), x.size(1), (int)x.size(1), stream());
-    const WgradPlan plan = wgrad_plan(n, (int)N, (int)K);
-    torch::Tensor part;
-    if (plan.part_floats > 0) part = torch::empty({plan.part_floats}, gp.options().dtype(torch::kFloat32));
-    check_launch(launch_wgrad(plan, static_cast<const char*>(gp.data_ptr()) + 2 * r0 * gp.stride(0), gp.stride(0),
-                              x.data_ptr(), x.size(1), n, (int)N, (int)K, dw.data_ptr(), dw.size(1),
-                              dw.scalar_type() == torch::kFloat32, r0 > 0,
-                              part.defined() ? part.data_ptr<float>() : nullptr, stream()),
-                 "weight_grad8");
+    run_wgrad(gp, N, r0, x, K, n, dw, r0 > 0);
   }
   if (dw.scalar_type() != dt) dw = dw.to(dt);
   return K % 8 == 0 ? dw : dw.narrow(1, 0, K);
@@ -406,12 +439,30 @@ struct SwiGLUNode : torch::autograd::Function<SwiGLUNode> {
 }  // namespace
 
 torch::Tensor norm(torch::Tensor x, OptTensor w, OptTensor b, double eps, bool layer, bool kept) {
+  if (w.has_value() && !w->is_contiguous()) w = w->contiguous();
+  if (b.has_value() && !b->is_contiguous()) b = b->contiguous();
   const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(w) || wants_grad(b));
   return NormNode::apply(x, w, b, eps, layer, kept && (x.requires_grad() || wants_grad(w)), grad);
 }
 
 // x, w, b: bf16 or fp32; computed in bf16.
 torch::Tensor linear8(torch::Tensor x, torch::Tensor w, OptTensor b) {
+  TORCH_CHECK_TYPE(x.is_cuda() && (x.scalar_type() == torch::kBFloat16 || x.scalar_type() == torch::kFloat32),
+                   "x must be bf16 or fp32 on CUDA, got ", type_text(x));
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x needs a last dimension of at least 1, got shape ",
+                    shape_text(x));
+  TORCH_CHECK_VALUE(w.dim() == 2 && w.size(1) == x.size(-1) && w.size(0) >= 1, "weight ", shape_text(w),
+                    " does not fit an input of width ", std::to_string(x.size(-1)));
+  TORCH_CHECK_VALUE(w.device() == x.device(), "weight is on ", device_text(w), ", the input on ", device_text(x));
+  TORCH_CHECK_TYPE(w.scalar_type() == torch::kBFloat16 || w.scalar_type() == torch::kFloat32,
+                   "weight must be bf16 or fp32, got ", type_text(w));
+  if (b.has_value()) {
+    TORCH_CHECK_VALUE(b->dim() == 1 && b->size(0) == w.size(0), "bias ", shape_text(*b), " does not fit a weight ",
+                      shape_text(w));
+    TORCH_CHECK_VALUE(b->device() == x.device(), "bias is on ", device_text(*b), ", the input on ", device_text(x));
+    TORCH_CHECK_TYPE(b->scalar_type() == torch::kBFloat16 || b->scalar_type() == torch::kFloat32,
+                     "bias must be bf16 or fp32, got ", type_text(*b));
+  }
   if (x.scalar_type() != torch::kBFloat16) x = x.to(torch::kBFloat16);
   const bool on = at::GradMode::is_enabled();
   return LinearNode::apply(x, w, b, on && w.requires_grad(), on && (x.requires_grad() || w.requires_grad() || wants_grad(b)));
@@ -429,10 +480,27 @@ torch::Tensor linear8_weight_grad(torch::Tensor g2, torch::Tensor codes, torch::
   return weight_grad8(operand(g2), g2.size(1), codes, scales, K, fp32);
 }
 
+// dW [N, K] = g [rows, N]^T x [rows, K] of bf16 matrices, in fp32 or bf16.
+torch::Tensor weight_grad(torch::Tensor g, torch::Tensor x, bool fp32) {
+  const at::cuda::CUDAGuard guard(g.device());
+  TORCH_CHECK(g.is_cuda() && x.is_cuda() && g.device() == x.device() && g.dim() == 2 && x.dim() == 2 &&
+                  g.scalar_type() == torch::kBFloat16 && x.scalar_type() == torch::kBFloat16 && g.size(0) == x.size(0) &&
+                  g.size(1) >= 1 && x.size(1) >= 1,
+              "weight_grad: g [rows, N] and x [rows, K] must be bf16 CUDA matrices of as many rows");
+  const int64_t rows = g.size(0), N = g.size(1), K = x.size(1);
+  const auto opt = g.options().dtype(fp32 ? torch::kFloat32 : torch::kBFloat16);
+  if (rows == 0) return torch::zeros({N, K}, opt);
+  auto dw = torch::empty({N, up8(K)}, opt);
+  run_wgrad(operand(g), N, 0, operand(x), K, rows, dw, false);
+  return K % 8 == 0 ? dw : dw.narrow(1, 0, K);
+}
+
 void bind_kept8(pybind11::module_& m) {
   const auto kNoGil = py::call_guard<py::gil_scoped_release>();
   m.def("keep8", &keep8, kNoGil);
   m.def("restore8", &restore8, kNoGil);
+  m.def("restore8_new", &restore8_new, kNoGil);
+  m.def("weight_grad", &weight_grad, kNoGil);
   m.def("swiglu8_fwd", &swiglu8_fwd, kNoGil);
   m.def("swiglu8_bwd", &swiglu8_bwd, kNoGil);
   m.def("swiglu8", &swiglu8, kNoGil);

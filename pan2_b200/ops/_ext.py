@@ -30,9 +30,11 @@ def ext():
     ) from _ERR
 
 
-# kernels launched by one call of each binding (for the benchmark's launch count)
+# kernels launched by one call of each binding (for the benchmark's launch count); the launches of the C++ autograd
+# nodes' backwards (norm, linear8, swiglu8) are not calls of a binding and not counted
 KERNELS_PER_CALL = {
-    "ln_modulate_bwd": 2, "gate_bwd": 2, "mse_fwd": 2, "attn_bwd": 3, "error_flag": 0,
+    "ln_modulate_bwd": 2, "gate_bwd": 2, "mse_fwd": 2, "attn_bwd": 3, "error_flag": 0, "linear8": 2,
+    "linear8_weight_grad": 2,
 }
 _COUNTING = {"on": False, "launches": 0, "by_name": {}}
 

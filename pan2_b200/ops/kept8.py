@@ -29,7 +29,7 @@ from typing import Optional, Tuple
 import torch
 
 from ._ext import ext
-from .gemm import _pad_k, mm_nn, mm_nt, mm_tn
+from .gemm import _pad_k, mm_nn, mm_nt
 
 BLOCK = 32
 
@@ -111,24 +111,14 @@ def keep_codes(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return ext().keep8(x) if x.is_cuda else _keep_cpu(x)
 
 
-def restore_codes(codes: torch.Tensor, scales: torch.Tensor, C: int, dtype: torch.dtype,
-                  row0: int = 0, rows: Optional[int] = None) -> torch.Tensor:
-    """Rows ``row0 : row0 + rows`` of the kept matrix as ``[rows, C]`` ``dtype``."""
-    rows = codes.shape[0] - row0 if rows is None else rows
-    if codes.is_cuda:
-        out = torch.empty(rows, C, dtype=dtype, device=codes.device)
-        ext().restore8(codes, scales, C, row0, out)
-        return out
-    return _values_cpu(codes[row0:row0 + rows], scales[row0:row0 + rows], C, dtype)
-
-
 # --------------------------------------------------------------------------------------------
 # store and reload
 # --------------------------------------------------------------------------------------------
 
 def keep8(x: torch.Tensor) -> Kept8:
     """``x`` (any leading dims and strides) held in 8 bits.  Not differentiable."""
-    check_activation(x, "x")
+    if not getattr(x, "is_cuda", False):  # the binding makes the same checks
+        check_activation(x, "x")
     return Kept8(*keep_codes(x), x.shape, x.dtype)
 
 
@@ -137,9 +127,11 @@ def restore8(kept: Kept8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     if not isinstance(kept, Kept8):
         raise TypeError(f"restore8 takes what keep8 returned, got {type(kept).__name__}")
     dtype = kept.dtype if dtype is None else dtype
-    if kept.codes.is_cuda and dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"restore8 gives bf16 or fp32 on CUDA, not {dtype}")
-    return restore_codes(kept.codes, kept.scales, kept.shape[-1], dtype).view(kept.shape)
+    if kept.codes.is_cuda:
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError(f"restore8 gives bf16 or fp32 on CUDA, not {dtype}")
+        return ext().restore8_new(kept.codes, kept.scales, kept.shape, dtype == torch.float32)
+    return _values_cpu(kept.codes, kept.scales, kept.shape[-1], dtype).view(kept.shape)
 
 
 # --------------------------------------------------------------------------------------------
@@ -249,9 +241,9 @@ def kept8_linear(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = N
 
     CUDA inputs compute in bf16 with fp32 accumulation, like :func:`pan2_b200.ops.gemm.linear`; any
     widths work (those that are not multiples of 8 are padded)."""
-    _check_linear(x, w, b)
-    if x.is_cuda:
+    if getattr(x, "is_cuda", False):  # the binding makes the same checks
         return ext().linear8(x, w, b)
+    _check_linear(x, w, b)
     return _Kept8LinearCPU.apply(x, w, b)
 
 
@@ -296,11 +288,11 @@ class _Kept8SwiGLUCPU(torch.autograd.Function):
 def kept8_swiglu(gate: torch.Tensor, value: torch.Tensor) -> torch.Tensor:
     """``silu(gate) * value``, computed in fp32 and rounded once, whose backward reads ``gate`` and
     ``value`` from 8 bits."""
+    if getattr(gate, "is_cuda", False) and getattr(value, "is_cuda", False):  # the binding makes the same checks
+        return ext().swiglu8(gate, value)
     check_activation(gate, "gate")
     check_activation(value, "value")
     _check_match(gate, value, "gate and value")
-    if gate.is_cuda:
-        return ext().swiglu8(gate, value)
     return _Kept8SwiGLUCPU.apply(gate, value)
 
 
@@ -333,14 +325,10 @@ class _Kept8SwiGLUFFN(torch.autograd.Function):
 
 
 def _dense_weight_grad(g2: torch.Tensor, h: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    if not g2.is_cuda:
-        wide = wide_dtype(g2.dtype)
-        return (g2.to(wide).t() @ h.to(wide)).to(dtype)
-    N, K = g2.shape[1], h.shape[1]
-    if g2.shape[0] == 0:
-        return torch.zeros(N, K, dtype=dtype, device=g2.device)
-    out_dtype = dtype if dtype == torch.bfloat16 else torch.float32
-    return mm_tn(_pad_k(g2, _pad8(N)), _pad_k(h, _pad8(K)), out_dtype=out_dtype)[:N, :K].to(dtype)
+    if g2.is_cuda:
+        return ext().weight_grad(g2, h, dtype != torch.bfloat16).to(dtype)
+    wide = wide_dtype(g2.dtype)
+    return (g2.to(wide).t() @ h.to(wide)).to(dtype)
 
 
 def kept8_swiglu_ffn(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Tensor) -> torch.Tensor:
@@ -354,4 +342,8 @@ def kept8_swiglu_ffn(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: to
         raise ValueError(f"output weight {tuple(w2.shape)} on {w2.device} does not fit a hidden width of {w1.shape[0]}")
     if x.is_cuda:
         x = x.to(torch.bfloat16)
+    if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, w1, w3, w2))):  # nothing to keep
+        x2 = x.reshape(-1, x.shape[-1])
+        h = kept8_swiglu(_project(x2, w1, None), _project(x2, w3, None))
+        return _project(h, w2, None).reshape(*x.shape[:-1], w2.shape[0])
     return _Kept8SwiGLUFFN.apply(x, w1, w3, w2)

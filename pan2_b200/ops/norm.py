@@ -73,8 +73,6 @@ def _check(x, w, b, eps):
             raise ValueError(f"{name} {tuple(t.shape)} does not fit rows of width {x.shape[-1]}")
         if t.device != x.device:
             raise ValueError(f"{name} is on {t.device}, x on {x.device}")
-        if x.is_cuda and t.dtype not in (torch.bfloat16, torch.float32):
-            raise TypeError(f"{name} must be bf16 or fp32, got {t.dtype}")
     if w is not None and b is not None and w.dtype != b.dtype:
         raise TypeError(f"weight and bias have different dtypes: {w.dtype} and {b.dtype}")
     if not eps >= 0:
@@ -82,15 +80,10 @@ def _check(x, w, b, eps):
 
 
 def _norm(x, w, b, eps, layer, kept8):
+    if getattr(x, "is_cuda", False):  # the binding makes the same checks
+        return ext().norm(x, w, b, eps, layer, kept8)
     _check(x, w, b, eps)
-    w, b = _flat(w), _flat(b)
-    if x.is_cuda:
-        return ext().norm(x, w, b, float(eps), layer, bool(kept8))
     return _NormCPU.apply(x, w, b, float(eps), layer, bool(kept8))
-
-
-def _flat(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,

@@ -393,6 +393,30 @@ def test_refusals():
         kept8_linear(x, torch.randn(8, 64))
     with pytest.raises(ValueError, match="differ"):
         kept8_swiglu(x, x.bfloat16())
+    with pytest.raises(ValueError, match="does not fit"):
+        layer_norm(x, torch.ones(32, device="cuda"))
+    with pytest.raises(ValueError, match="does not fit"):
+        layer_norm(x, torch.ones(64, device="cuda"), torch.ones(63, device="cuda"))
+    with pytest.raises(TypeError, match="different dtypes"):
+        layer_norm(x, torch.ones(64, device="cuda"), torch.ones(64, device="cuda").bfloat16())
+    with pytest.raises(ValueError, match="negative"):
+        rms_norm(x, eps=-1.0)
+    with pytest.raises(ValueError, match="last dimension"):
+        keep8(torch.zeros(4, 0, device="cuda"))
+    with pytest.raises(ValueError, match="last dimension"):
+        rms_norm(torch.tensor(1.0, device="cuda"))
+    with pytest.raises(ValueError, match="does not fit"):
+        kept8_linear(x, torch.randn(8, 32, device="cuda"))
+    with pytest.raises(ValueError, match="does not fit"):
+        kept8_linear(x, torch.randn(8, 64, device="cuda"), torch.randn(9, device="cuda"))
+    with pytest.raises(TypeError, match="bf16 or fp32"):
+        kept8_linear(x, torch.randn(8, 64, device="cuda").half())
+    with pytest.raises(ValueError, match="differ"):
+        kept8_swiglu(x, torch.randn(4, 32, device="cuda"))
+    with pytest.raises(ValueError, match="differ"):
+        kept8_swiglu(x, x.cpu())
+    with pytest.raises(ValueError, match="does not fit"):
+        kept8_swiglu_ffn(x, torch.randn(8, 64, device="cuda"), torch.randn(8, 64, device="cuda"), torch.randn(64, 9, device="cuda"))
     kept = keep8(x)
     from pan2_b200.ops._ext import ext
     with pytest.raises(RuntimeError, match="rows out of range"):
