@@ -4,7 +4,7 @@
 // All kernels here are element streams bounded by DRAM.  Work is cut into fragments of V elements; the 32 / V lanes
 // that hold one block of 32 agree on its scale by shuffles, so every input is read once.  Three forms:
 //   V = 8   C % 8 == 0 and every row 16-byte aligned: 16-byte accesses
-//   flat    contiguous tensors of any other width: tiles through shared memory (flat.cuh), V = 4 there
+//   flat    contiguous tensors of any other width: tiles through shared memory (flat.cuh), fragments of 4 or 8
 //   V = 1   what is left (odd views): one element a lane
 #include "flat.cuh"
 #include "kept8.cuh"
@@ -150,11 +150,12 @@ __global__ void __launch_bounds__(kThreads) restore8_kernel(Units un, Kept8Out k
 
 // ---------------------------------------------------------------- SwiGLU
 // 1 / (1 + exp(-g)) by the hardware's base-2 exponential and reciprocal: their errors, and |g| 2^-24 from the
-// product with log2(e), reach the result times s (1 - s), below 2^-22 everywhere.  exp(-g) = inf gives 0.
+// product with log2(e), reach the result times s (1 - s), below 2^-22 everywhere.  exp(-g) = inf gives 0, and what
+// would be subnormal is 0 (the forms that keep subnormals take several instructions more each).
 __device__ __forceinline__ float sigmoid_fast(float g) {
   float e, s;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
-  asm("rcp.approx.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
   return s;
 }
 
@@ -235,9 +236,14 @@ __global__ void __launch_bounds__(kThreads) swiglu_bwd_kernel(RowView dh, Kept8O
 }
 
 // ---------------------------------------------------------------- flat form
-// A tile is kFlatTile elements of whole rows, or of one row when that is longer.  Lane groups of eight hold a block, four
-// elements a lane; a tile's fragments are (row, 4 columns) over rows padded to whole blocks.
-constexpr int kFlatTile = 4096;
+// A tile is 16 KB of whole rows, or of one row when that is longer.  Its fragments are (row, V columns) over rows padded
+// to whole blocks, 32 / V lanes to a block.  V = 8 for bf16, where the kernels are bound by instructions: keep8 of 200001 x
+// 1001 took 242 us with 4 columns and 8 KB tiles, 190 with 8, 172 with the packed encoding, 156 with 16 KB tiles (3.9 TB/s).
+// V = 4 for fp32, where 8 would read shared memory at half the rate.
+constexpr int flat_v(bool fp32) { return fp32 ? 4 : 8; }
+constexpr int flat_size(bool fp32) { return fp32 ? 4096 : 8192; }  // 16 KB
+template <typename T>
+constexpr bool is_fp32() { return sizeof(T) == 4; }
 
 struct FlatTiles {
   FastDiv per_row, frag_row;  // tiles a row (1 unless rows are long), fragments a padded row of a tile
@@ -251,7 +257,9 @@ struct FlatTile {
   uint32_t frags;    // fragments of the tile
 };
 
+template <typename T>
 __device__ __forceinline__ FlatTile flat_tile(const FlatTiles& t) {
+  constexpr int V = flat_v(is_fp32<T>()), SIZE = flat_size(is_fp32<T>());
   FlatTile f;
   if (t.rows > 1 || t.per_row.d == 1) {
     f.row0 = blockIdx.x * t.rows;
@@ -261,57 +269,83 @@ __device__ __forceinline__ FlatTile flat_tile(const FlatTiles& t) {
   } else {
     f.row0 = t.per_row.div(blockIdx.x);
     f.rows = 1;
-    f.c0 = (int)(blockIdx.x - f.row0 * t.per_row.d) * kFlatTile;
-    f.cols = min(kFlatTile, t.C - f.c0);
+    f.c0 = (int)(blockIdx.x - f.row0 * t.per_row.d) * SIZE;
+    f.cols = min(SIZE, t.C - f.c0);
   }
-  f.frags = f.rows * ((f.cols + kKeptBlock - 1) / kKeptBlock * (kKeptBlock / 4));
+  f.frags = f.rows * ((f.cols + kKeptBlock - 1) / kKeptBlock * (kKeptBlock / V));
   return f;
 }
 
 // Fragment u of the tile: its row (in the tile) and first column (in the tile).
+template <int V>
 __device__ __forceinline__ void flat_frag(const FlatTiles& t, const FlatTile& f, uint32_t u, uint32_t& r, int& c) {
   r = f.rows == 1 ? 0 : t.frag_row.div(u);
-  c = (int)(u - r * t.frag_row.d) * 4;
+  c = (int)(u - r * t.frag_row.d) * V;
 }
 
-template <typename T>
-__device__ __forceinline__ void flat_read(const uint8_t* smem, const FlatTile& f, uint32_t r, int c, float (&v)[4]) {
+template <typename T, int V>
+__device__ __forceinline__ void flat_read(const uint8_t* smem, const FlatTile& f, uint32_t r, int c, float (&v)[V]) {
   const T* p = reinterpret_cast<const T*>(smem) + r * f.cols + c;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = c + i < f.cols ? to_f32(p[i]) : 0.f;
+  for (int i = 0; i < V; ++i) v[i] = c + i < f.cols ? to_f32(p[i]) : 0.f;
 }
-template <typename T>
-__device__ __forceinline__ void flat_write(uint8_t* smem, const FlatTile& f, uint32_t r, int c, const float (&v)[4]) {
+template <typename T, int V>
+__device__ __forceinline__ void flat_write(uint8_t* smem, const FlatTile& f, uint32_t r, int c, const float (&v)[V]) {
   T* p = reinterpret_cast<T*>(smem) + r * f.cols + c;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < V; ++i)
     if (c + i < f.cols) p[i] = from_f32<T>(v[i]);
 }
 
+// Eight bf16 as they would lie in an aligned row.
+__device__ __forceinline__ Frag<__nv_bfloat16> flat_frag8(const uint8_t* smem, const FlatTile& f, uint32_t r, int c) {
+  const uint16_t* p = reinterpret_cast<const uint16_t*>(smem) + r * f.cols + c;
+  uint32_t e[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = c + i < f.cols ? p[i] : 0u;
+  Frag<__nv_bfloat16> x;
+  x.raw = make_uint4(__byte_perm(e[0], e[1], 0x5410), __byte_perm(e[2], e[3], 0x5410), __byte_perm(e[4], e[5], 0x5410),
+                     __byte_perm(e[6], e[7], 0x5410));
+  return x;
+}
+
 // Scale and codes of a fragment; all lanes of the warp take part, `act` lanes store.
-__device__ __forceinline__ void flat_keep(const Kept8Out& o, uint32_t row, int c, bool act, const float (&v)[4]) {
+template <int V>
+__device__ __forceinline__ void flat_keep(const Kept8Out& o, uint32_t row, int c, bool act, const float (&v)[V]) {
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
 #pragma unroll
-  for (int d = 1; d < 8; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  for (int d = 1; d < kKeptBlock / V; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
   const uint32_t b = kept8_byte(m);
   if (!act) return;
   const float inv = kept8_inv_step(b);
-  *reinterpret_cast<uint32_t*>(o.codes + (long long)row * o.Cp + c) =
-      pack4_low_bytes(kept8_code(v[0], inv), kept8_code(v[1], inv), kept8_code(v[2], inv), kept8_code(v[3], inv));
+  uint32_t w[V / 4];
+#pragma unroll
+  for (int i = 0; i < V / 4; ++i)
+    w[i] = pack4_low_bytes(kept8_code(v[4 * i], inv), kept8_code(v[4 * i + 1], inv), kept8_code(v[4 * i + 2], inv),
+                           kept8_code(v[4 * i + 3], inv));
+  int8_t* at = o.codes + (long long)row * o.Cp + c;
+  if constexpr (V == 8) *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(at) = w[0];
   if (c % kKeptBlock == 0) kept8_store_byte(o.scales + (long long)row * o.nbp, c / kKeptBlock, o.nb, o.nbp, b);
 }
 
-__device__ __forceinline__ void flat_values(const Kept8Out& k, uint32_t row, int c, float (&v)[4]) {
-  const uint32_t w = *reinterpret_cast<const uint32_t*>(k.codes + (long long)row * k.Cp + c) ^ 0x80808080u;
+template <int V>
+__device__ __forceinline__ void flat_values(const Kept8Out& k, uint32_t row, int c, float (&v)[V]) {
+  const int8_t* at = k.codes + (long long)row * k.Cp + c;
   const float step = kept8_step(k.scales[(long long)row * k.nbp + c / kKeptBlock]);
+  if constexpr (V == 8) {
+    kept8_values(*reinterpret_cast<const uint2*>(at), step, v);
+  } else {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(at) ^ 0x80808080u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 + i)) - 8388736.f) * step;
+    for (int i = 0; i < 4; ++i) v[i] = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 + i)) - 8388736.f) * step;
+  }
 }
 
 template <typename T>
-constexpr uint32_t flat_room() { return FlatRun<T>::room(kFlatTile); }
+constexpr uint32_t flat_room() { return FlatRun<T>::room(flat_size(is_fp32<T>())); }
 __device__ __forceinline__ void flat_wait() {
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
@@ -324,42 +358,46 @@ __device__ __forceinline__ FlatRun<T> flat_run(const void* p, const FlatTiles& t
 template <typename T>
 __global__ void __launch_bounds__(kThreads) keep8_flat_kernel(const T* x, FlatTiles t, Kept8Out o, T* __restrict__ copy,
                                                               long long ld) {
+  constexpr int V = flat_v(is_fp32<T>());
   __shared__ __align__(16) uint8_t sx[flat_room<T>()];
-  const FlatTile f = flat_tile(t);
+  const FlatTile f = flat_tile<T>(t);
   const FlatRun<T> run = flat_run<T>(x, t, f);
   run.fetch(sx);
   flat_wait();
-  for (uint32_t u0 = 0; u0 < f.frags; u0 += kThreads) {  // whole warps: a tile's fragments are a multiple of 8
+  for (uint32_t u0 = 0; u0 < f.frags; u0 += kThreads) {  // whole warps: a block's lanes are in or out together
     const uint32_t u = u0 + threadIdx.x;
     const bool act = u < f.frags;
     uint32_t r;
     int c;
-    flat_frag(t, f, act ? u : 0, r, c);
-    float v[4];
-    flat_read<T>(sx + run.head, f, r, c, v);
+    flat_frag<V>(t, f, act ? u : 0, r, c);
     const uint32_t row = f.row0 + r;
-    flat_keep(o, row, f.c0 + c, act, v);
     if constexpr (sizeof(T) == 2) {
-      if (copy != nullptr && act && f.c0 + c < ld)  // ld % 8 == 0: the four columns are inside
-        *reinterpret_cast<uint2*>(copy + (long long)row * ld + f.c0 + c) =
-            make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+      Piece<T, 8> piece;
+      piece.f = flat_frag8(sx + run.head, f, r, c);
+      keep_fragment<T, 8>(o, row, f.c0 + c, act, piece);
+      if (copy != nullptr && act && f.c0 + c < ld) piece.store(copy + (long long)row * ld + f.c0 + c);  // ld % 8 == 0
+    } else {
+      float v[V];
+      flat_read<T, V>(sx + run.head, f, r, c, v);
+      flat_keep(o, row, f.c0 + c, act, v);
     }
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) restore8_flat_kernel(FlatTiles t, Kept8Out k, T* __restrict__ out) {
+  constexpr int V = flat_v(is_fp32<T>());
   __shared__ __align__(16) uint8_t so[flat_room<T>()];
-  const FlatTile f = flat_tile(t);
+  const FlatTile f = flat_tile<T>(t);
   const FlatRun<T> run = flat_run<T>(out, t, f);
 #pragma unroll 2
   for (uint32_t u = threadIdx.x; u < f.frags; u += kThreads) {
     uint32_t r;
     int c;
-    flat_frag(t, f, u, r, c);
-    float v[4];
+    flat_frag<V>(t, f, u, r, c);
+    float v[V];
     flat_values(k, f.row0 + r, f.c0 + c, v);
-    flat_write<T>(so + run.head, f, r, c, v);
+    flat_write<T, V>(so + run.head, f, r, c, v);
   }
   __syncthreads();
   run.store(so);
@@ -368,8 +406,9 @@ __global__ void __launch_bounds__(kThreads) restore8_flat_kernel(FlatTiles t, Ke
 template <typename T>
 __global__ void __launch_bounds__(kThreads) swiglu_fwd_flat_kernel(const T* gate, const T* value, FlatTiles t,
                                                                    Kept8Out og, Kept8Out ov, T* __restrict__ h) {
+  constexpr int V = flat_v(is_fp32<T>());
   __shared__ __align__(16) uint8_t sg[flat_room<T>()], sv[flat_room<T>()];
-  const FlatTile f = flat_tile(t);
+  const FlatTile f = flat_tile<T>(t);
   const FlatRun<T> rg = flat_run<T>(gate, t, f), rv = flat_run<T>(value, t, f), rh = flat_run<T>(h, t, f);
   rg.fetch(sg);
   rv.fetch(sv);
@@ -379,18 +418,33 @@ __global__ void __launch_bounds__(kThreads) swiglu_fwd_flat_kernel(const T* gate
     const bool act = u < f.frags;
     uint32_t r;
     int c;
-    flat_frag(t, f, act ? u : 0, r, c);
-    float g[4], v[4];
-    flat_read<T>(sg + rg.head, f, r, c, g);
-    flat_read<T>(sv + rv.head, f, r, c, v);
-    if (og.codes != nullptr) {
-      flat_keep(og, f.row0 + r, f.c0 + c, act, g);
-      flat_keep(ov, f.row0 + r, f.c0 + c, act, v);
+    flat_frag<V>(t, f, act ? u : 0, r, c);
+    float g[V], v[V];
+    if constexpr (sizeof(T) == 2) {
+      Piece<T, 8> pg, pv;
+      pg.f = flat_frag8(sg + rg.head, f, r, c);
+      pv.f = flat_frag8(sv + rv.head, f, r, c);
+      if (og.codes != nullptr) {
+        keep_fragment<T, 8>(og, f.row0 + r, f.c0 + c, act, pg);
+        keep_fragment<T, 8>(ov, f.row0 + r, f.c0 + c, act, pv);
+      }
+      float2 a[4], b[4];
+      pg.get(a);
+      pv.get(b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) g[2 * i] = a[i].x, g[2 * i + 1] = a[i].y, v[2 * i] = b[i].x, v[2 * i + 1] = b[i].y;
+    } else {
+      flat_read<T, V>(sg + rg.head, f, r, c, g);
+      flat_read<T, V>(sv + rv.head, f, r, c, v);
+      if (og.codes != nullptr) {
+        flat_keep(og, f.row0 + r, f.c0 + c, act, g);
+        flat_keep(ov, f.row0 + r, f.c0 + c, act, v);
+      }
     }
     if (!act) continue;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= g[i] * sigmoid_fast(g[i]);
-    flat_write<T>(sv + rv.head, f, r, c, v);  // h takes the place of value: same offsets, own elements
+    for (int i = 0; i < V; ++i) v[i] *= g[i] * sigmoid_fast(g[i]);
+    flat_write<T, V>(sv + rv.head, f, r, c, v);  // h takes the place of value: same offsets, own elements
   }
   __syncthreads();
   rh.store(sv);
@@ -400,8 +454,9 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) swiglu_bwd_flat_kernel(const T* dh, Kept8Out kg, Kept8Out kv, FlatTiles t,
                                                                    T* __restrict__ dgate, T* __restrict__ dvalue,
                                                                    T* __restrict__ h) {
+  constexpr int V = flat_v(is_fp32<T>());
   __shared__ __align__(16) uint8_t sd[flat_room<T>()], sv[flat_room<T>()];
-  const FlatTile f = flat_tile(t);
+  const FlatTile f = flat_tile<T>(t);
   const FlatRun<T> rd = flat_run<T>(dh, t, f);
   rd.fetch(sd);
   flat_wait();
@@ -409,25 +464,25 @@ __global__ void __launch_bounds__(kThreads) swiglu_bwd_flat_kernel(const T* dh, 
     for (uint32_t u = threadIdx.x; u < f.frags; u += kThreads) {
       uint32_t r;
       int c;
-      flat_frag(t, f, u, r, c);
-      float g[4], w[4];
+      flat_frag<V>(t, f, u, r, c);
+      float g[V], w[V];
       flat_values(kg, f.row0 + r, f.c0 + c, g);
       flat_values(kv, f.row0 + r, f.c0 + c, w);
       if (pass == 0) {
-        float d[4], o[4];
-        flat_read<T>(sd + rd.head, f, r, c, d);
+        float d[V], o[V];
+        flat_read<T, V>(sd + rd.head, f, r, c, d);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < V; ++i) {
           const float s = sigmoid_fast(g[i]), ds = d[i] * s;
           o[i] = ds * w[i] * fmaf(g[i], 1.f - s, 1.f);
           d[i] = ds * g[i];
         }
-        flat_write<T>(sd + rd.head, f, r, c, o);
-        flat_write<T>(sv + rd.head, f, r, c, d);
+        flat_write<T, V>(sd + rd.head, f, r, c, o);
+        flat_write<T, V>(sv + rd.head, f, r, c, d);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] *= g[i] * sigmoid_fast(g[i]);
-        flat_write<T>(sd + rd.head, f, r, c, w);
+        for (int i = 0; i < V; ++i) w[i] *= g[i] * sigmoid_fast(g[i]);
+        flat_write<T, V>(sd + rd.head, f, r, c, w);
       }
     }
     __syncthreads();
@@ -563,19 +618,19 @@ bool contiguous_rows(const RowsArg& a, int C) {
   return a.inner == 1 && a.outer_stride == C && reinterpret_cast<uintptr_t>(a.p) % 16 == 0;
 }
 
-FlatTiles flat_tiles(long long rows, int C, uint32_t* grid) {
+FlatTiles flat_tiles(long long rows, int C, bool fp32, uint32_t* grid) {
   FlatTiles t;
-  const int tiles = (C + kFlatTile - 1) / kFlatTile;
+  const int size = flat_size(fp32), tiles = (C + size - 1) / size;
   t.per_row = FastDiv((uint32_t)tiles);
-  t.rows = tiles > 1 ? 1 : kFlatTile / C;
+  t.rows = tiles > 1 ? 1 : size / C;
   t.C = C;
-  t.frag_row = FastDiv((uint32_t)((tiles > 1 ? kFlatTile : (C + kKeptBlock - 1) / kKeptBlock * kKeptBlock) / 4));
+  t.frag_row = FastDiv((uint32_t)((tiles > 1 ? size : (C + kKeptBlock - 1) / kKeptBlock * kKeptBlock) / flat_v(fp32)));
   t.total_rows = (uint32_t)rows;
   *grid = tiles > 1 ? (uint32_t)rows * (uint32_t)tiles : (uint32_t)((rows + t.rows - 1) / t.rows);
   return t;
 }
 // Tiles are counted in 31 bits.
-bool flat_fits(long long rows, int C) { return rows * ((C + kFlatTile - 1) / kFlatTile) < (1ll << 31); }
+bool flat_fits(long long rows, int C) { return rows * ((C + 4095) / 4096) < (1ll << 31); }
 
 // 16-byte fragments: C in whole fragments and every row start aligned.
 bool fragments_of_8(const RowsArg& a, int C, bool fp32) {
@@ -602,7 +657,7 @@ void launch_keep8(const RowsArg& x, long long rows, bool fp32, const Kept8Buf& k
   const bool vec = fragments_of_8(x, k.C, fp32);
   if (!vec && contiguous_rows(x, k.C) && flat_fits(rows, k.C)) {
     uint32_t grid;
-    const FlatTiles t = flat_tiles(rows, k.C, &grid);
+    const FlatTiles t = flat_tiles(rows, k.C, fp32, &grid);
     if (fp32) keep8_flat_kernel<float><<<grid, kThreads, 0, s>>>((const float*)x.p, t, out_of(k), (float*)copy, ld);
     else keep8_flat_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>((const __nv_bfloat16*)x.p, t, out_of(k), (__nv_bfloat16*)copy, ld);
     return;
@@ -619,7 +674,7 @@ void launch_restore8(const Kept8Buf& k, long long row0, long long rows, bool fp3
   const bool vec = fragments_of_8(o, cols, fp32);
   if (!vec && cols == k.C && contiguous_rows(o, k.C) && flat_fits(rows, k.C)) {
     uint32_t grid;
-    const FlatTiles t = flat_tiles(rows, k.C, &grid);
+    const FlatTiles t = flat_tiles(rows, k.C, fp32, &grid);
     Kept8Out from = out_of(k);
     from.codes += row0 * from.Cp;
     from.scales += row0 * from.nbp;
@@ -638,7 +693,7 @@ void launch_swiglu_fwd(const RowsArg& g, const RowsArg& v, long long rows, bool 
   const bool vec = fragments_of_8(g, kg.C, fp32) && fragments_of_8(v, kg.C, fp32);
   if (!vec && contiguous_rows(g, kg.C) && contiguous_rows(v, kg.C) && flat_fits(rows, kg.C)) {
     uint32_t grid;
-    const FlatTiles t = flat_tiles(rows, kg.C, &grid);
+    const FlatTiles t = flat_tiles(rows, kg.C, fp32, &grid);
     if (fp32)
       swiglu_fwd_flat_kernel<float><<<grid, kThreads, 0, s>>>((const float*)g.p, (const float*)v.p, t, out_of(kg),
                                                               out_of(kv), (float*)h);
@@ -658,7 +713,7 @@ void launch_swiglu_bwd(const RowsArg& dh, long long rows, bool fp32, const Kept8
   const bool vec = fragments_of_8(dh, kg.C, fp32);
   if (!vec && contiguous_rows(dh, kg.C) && flat_fits(rows, kg.C)) {
     uint32_t grid;
-    const FlatTiles t = flat_tiles(rows, kg.C, &grid);
+    const FlatTiles t = flat_tiles(rows, kg.C, fp32, &grid);
     if (fp32)
       swiglu_bwd_flat_kernel<float><<<grid, kThreads, 0, s>>>((const float*)dh.p, out_of(kg), out_of(kv), t, (float*)dg,
                                                               (float*)dv, (float*)h);
