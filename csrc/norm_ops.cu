@@ -13,7 +13,7 @@
 // registers, and one partial row of dw / db per CTA goes to scratch, which a second kernel adds up in order (no
 // atomics: the same bits every time).  Four forms:
 //   staged   (C % 8 == 0, 16-byte aligned rows, C <= 16384)  8-column fragments through rings in shared memory
-//   flat     (contiguous rows of other widths, C <= 8192)    batches of rows as one run of bytes (flat.cuh)
+//   flat     (contiguous rows of other widths, C <= 8192)    batches of rows as runs of bytes (flat.cuh)
 //   single   (other views, C <= 8192)                        one column at a time, straight from memory
 //   wide     (wider rows)                                    CTA per row, the row swept from memory
 // Groups of up to a warp reduce by shuffles, larger ones through shared memory.
@@ -498,11 +498,11 @@ __global__ void __launch_bounds__(threads_of(G), CTAS)
 }
 
 // ---------------------------------------------------------------- flat form
-// A batch is GROUPS * R neighbouring rows, one run of bytes; the next two or three arrive while one is worked on (one
+// Rows of up to 1024 columns.  A batch is GROUPS * R neighbouring rows, one run of bytes; the next two or three arrive while one is worked on (one
 // ahead left the kernel waiting for memory at 35 % of its bandwidth).  Fragment i of thread t are the 4 columns from 4 (t + i G) on: eight lanes hold a block of
 // the codes.  Results take the place of the input and leave as one run.
-constexpr int flat_ctas(int G, int R) { return threads_of(G) > 256 ? 1 : R == 1 ? 3 : 2; }
-constexpr int flat_depth(int G) { return 3; }
+constexpr int kGroupCtas = 2;
+constexpr int kGroupDepth = 3;
 
 template <typename T, int G, int UPT, int R>
 struct FlatBatch {
@@ -526,7 +526,7 @@ __device__ __forceinline__ void write4(T* p, int n, const float (&v)[4]) {
 }
 
 template <typename T, int G, int UPT, int R>
-__global__ void __launch_bounds__(threads_of(G), flat_ctas(G, R))
+__global__ void __launch_bounds__(threads_of(G), kGroupCtas)
     norm_fwd_flat_kernel(const T* x, uint32_t rows, int C, Vectors vec, float eps, bool layer, T* __restrict__ y,
                          float* __restrict__ stats, Kept k) {
   using B = FlatBatch<T, G, UPT, R>;
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(threads_of(G), flat_ctas(G, R))
   };
   const uint64_t step = (uint64_t)gridDim.x * B::ROWS;
   uint64_t r0 = (uint64_t)blockIdx.x * B::ROWS;
-  constexpr int DEPTH = flat_depth(G);
+  constexpr int DEPTH = kGroupDepth;
 #pragma unroll
   for (int d = 0; d < DEPTH - 1; ++d) {
     if (r0 + d * step < rows) run_of(x, r0 + d * step).fetch(ring + d * B::ROOM);
@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(threads_of(G), flat_ctas(G, R))
 }
 
 template <typename T, int G, int UPT, int R, bool KEPT>
-__global__ void __launch_bounds__(threads_of(G), flat_ctas(G, R))
+__global__ void __launch_bounds__(threads_of(G), kGroupCtas)
     norm_bwd_flat_kernel(const T* dy, const T* x, Kept k, uint32_t rows, int C, Vectors vec, bool layer,
                          const float* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, void* dw,
                          void* db) {
@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(threads_of(G), flat_ctas(G, R))
   };
   const uint64_t step = (uint64_t)gridDim.x * B::ROWS;
   uint64_t r0 = (uint64_t)blockIdx.x * B::ROWS;
-  constexpr int DEPTH = flat_depth(G);
+  constexpr int DEPTH = kGroupDepth;
 #pragma unroll
   for (int d = 0; d < DEPTH - 1; ++d) {
     if (r0 + d * step < rows) fetch(r0 + d * step, ring + d * STAGE);
@@ -751,6 +751,222 @@ __global__ void __launch_bounds__(threads_of(G), flat_ctas(G, R))
       store_partial(aw[i * 4 + j], (t + i * G) * 4 + j, C, 0, vec.fp32, part, dw);
       store_partial(ab[i * 4 + j], (t + i * G) * 4 + j, C, 1, vec.fp32, part, db);
     }
+  }
+}
+
+// ---------------------------------------------------------------- flat form, long rows
+// Row sums are taken by whole warps, a row each (or `segs` warps a row where few rows fit): no barrier and no idle threads
+// per row.  Lanes read neighbouring columns, so odd widths cost no bank conflicts, and a warp's 32 columns are one block of
+// the codes.  Measured against the groups above, which hold a row in registers and reduce with a barrier: 40000 x 2169 bf16
+// kept forward 540 / 262 us, backward 601 / 327; 40000 x 1501 167 / 178 and 212 / 190; 100000 x 1001 198 / 325 and 251 / 287; so
+// rows of up to 1024 columns take the groups.
+constexpr int kFlatDepth = 2;
+struct FlatPlan {
+  int rows, segs;          // rows of a batch; warps a row
+  uint32_t room, codes, scales;  // bytes of a stage for a tensor, the codes, the scales
+  uint32_t stage, vectors; // bytes of a stage; offset of the fp32 weight (and bias)
+};
+
+// Sum over a row's columns [c0, c1) of f(c), by one warp; every lane gets it.
+template <typename F>
+__device__ __forceinline__ float row_sum(int c0, int c1, F&& f) {
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  const int lane = threadIdx.x & 31;
+  int c = c0 + lane;
+  for (; c + 96 < c1; c += 128) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] += f(c + 32 * j);
+  }
+  for (; c < c1; c += 32) acc[0] += f(c);
+  return warp_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
+}
+
+// Sum of the row's segments; `part` holds segs values of the row, written by their warps.
+__device__ __forceinline__ float join_segs(float v, float* part, int seg, int segs) {
+  if (segs == 1) return v;
+  if ((threadIdx.x & 31) == 0) part[seg] = v;
+  __syncthreads();
+  v = 0.f;
+  for (int i = 0; i < segs; ++i) v += part[i];
+  return v;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2)
+    norm_fwd_long_kernel(const T* x, uint32_t rows, int C, Vectors vec, float eps, bool layer, T* __restrict__ y,
+                         float* __restrict__ stats, Kept k, FlatPlan pl) {
+  constexpr int WARPS = kThreads / 32;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float parts[2][WARPS];
+  float* w = reinterpret_cast<float*>(ring + pl.vectors);
+  float* b = w + C;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto run_of = [&](const T* p, uint64_t r0) {
+    return FlatRun<T>(p, (long long)r0 * C, (uint32_t)min((uint64_t)pl.rows, rows - r0) * C);
+  };
+  const uint64_t step = (uint64_t)gridDim.x * pl.rows;
+  uint64_t r0 = (uint64_t)blockIdx.x * pl.rows;
+  if (r0 < rows) run_of(x, r0).fetch(ring);
+  copy_commit();
+  for (int c = threadIdx.x; c < C; c += kThreads) {
+    w[c] = vec_at(vec.w, vec.fp32, c, 1.f);
+    b[c] = vec_at(vec.b, vec.fp32, c, 0.f);
+  }
+  const float inv_c = 1.f / C;
+  const int width = pl.segs == 1 ? C : ((C + pl.segs - 1) / pl.segs + 31) / 32 * 32;  // columns of a segment, whole blocks
+  for (int stage = 0; r0 < rows; r0 += step, stage ^= 1) {
+    if (r0 + step < rows) run_of(x, r0 + step).fetch(ring + (stage ^ 1) * pl.stage);
+    copy_commit();
+    copy_wait<1>();
+    __syncthreads();
+    uint8_t* at = ring + stage * pl.stage;
+    T* tile = reinterpret_cast<T*>(at + run_of(x, r0).head);
+    // with segments every warp has one unit, so that all take the barriers
+    for (int u = warp; u < pl.rows * pl.segs; u += WARPS) {
+      const int row = u / pl.segs, seg = u % pl.segs;
+      const bool in = r0 + row < rows;
+      if (!in && pl.segs == 1) break;
+      T* xr = tile + row * C;
+      const int c0 = min(C, seg * width), c1 = in ? min(C, c0 + width) : c0;
+      float mean = 0.f;
+      if (layer)
+        mean = join_segs(row_sum(c0, c1, [&](int c) { return to_f32(xr[c]); }), &parts[0][row * pl.segs], seg, pl.segs) * inv_c;
+      const float var = join_segs(row_sum(c0, c1, [&](int c) {
+        const float d = to_f32(xr[c]) - mean;
+        return d * d;
+      }), &parts[1][row * pl.segs], seg, pl.segs);
+      if (!in) continue;
+      const uint64_t r = r0 + row;
+      const float rstd = rsqrtf(var * inv_c + eps);
+      if (lane == 0 && seg == 0 && stats != nullptr) *reinterpret_cast<float2*>(stats + 2 * r) = make_float2(mean, rstd);
+      int8_t* codes = k.codes + (long long)r * k.Cp;
+      uint8_t* scales = k.scales + (long long)r * k.nbp;
+#pragma unroll 4
+      for (int cb = c0; cb < c1; cb += 32) {
+        const int c = cb + lane;
+        const float v[1] = {c < c1 ? to_f32(xr[c]) : 0.f};
+        if (k.codes != nullptr) {
+          const uint32_t sb = kept8_byte(kept8_amax<1>(v));
+          kept8_store_codes<1>(codes + c, v, sb);
+          if (lane == 0) kept8_store_byte(scales, cb / kKeptBlock, k.nb, k.nbp, sb);
+        }
+        if (c < c1) xr[c] = from_f32<T>(fmaf((v[0] - mean) * rstd, w[c], b[c]));
+      }
+    }
+    __syncthreads();
+    run_of(y, r0).store(at);  // y is aligned as x is: the same offsets
+    __syncthreads();
+  }
+}
+
+// Phase 1, warps: the sums of each row.  Phase 2, threads: columns t + i NT of all rows, dw and db in registers, dx over dy.
+template <typename T, int NT, int E, bool KEPT>
+__global__ void __launch_bounds__(NT, NT == 256 ? 2 : 1)
+    norm_bwd_long_kernel(const T* dy, const T* x, Kept k, uint32_t rows, int C, Vectors vec, bool layer,
+                         const float* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, void* dw,
+                         void* db, FlatPlan pl) {
+  constexpr int WARPS = NT / 32;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float parts[2][WARPS];
+  float* w = reinterpret_cast<float*>(ring + pl.vectors);
+  float4* row_of = reinterpret_cast<float4*>(w + (C + 3) / 4 * 4);  // (mean, rstd, a, b) of each row
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t X0 = pl.room, S0 = X0 + (KEPT ? pl.codes : pl.room);
+  auto count = [&](uint64_t r0) { return (uint32_t)min((uint64_t)pl.rows, rows - r0); };
+  auto fetch = [&](uint64_t r0, uint8_t* at) {
+    FlatRun<T>(dy, (long long)r0 * C, count(r0) * C).fetch(at);
+    if constexpr (KEPT) {
+      FlatRun<int8_t>(k.codes, (long long)r0 * k.Cp, count(r0) * k.Cp).fetch(at + X0);
+      FlatRun<uint8_t>(k.scales, (long long)r0 * k.nbp, count(r0) * k.nbp).fetch(at + S0);
+    } else {
+      FlatRun<T>(x, (long long)r0 * C, count(r0) * C).fetch(at + X0);
+    }
+  };
+  const uint64_t step = (uint64_t)gridDim.x * pl.rows;
+  uint64_t r0 = (uint64_t)blockIdx.x * pl.rows;
+  if (r0 < rows) fetch(r0, ring);
+  copy_commit();
+  for (int c = threadIdx.x; c < C; c += NT) w[c] = vec_at(vec.w, vec.fp32, c, 1.f);
+  const int t = threadIdx.x;
+  float aw[E], ab[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) aw[i] = ab[i] = 0.f;
+  const float inv_c = 1.f / C;
+  const int width = pl.segs == 1 ? C : ((C + pl.segs - 1) / pl.segs + 31) / 32 * 32;
+  for (int stage = 0; r0 < rows; r0 += step, stage ^= 1) {
+    if (r0 + step < rows) fetch(r0 + step, ring + (stage ^ 1) * pl.stage);
+    copy_commit();
+    copy_wait<1>();
+    __syncthreads();
+    uint8_t* at = ring + stage * pl.stage;
+    const uint32_t head = FlatRun<T>(dy, (long long)r0 * C, 0).head;
+    T* gt = reinterpret_cast<T*>(at + head);
+    const T* xt = reinterpret_cast<const T*>(at + X0 + head);
+    const int8_t* ct = reinterpret_cast<const int8_t*>(at + X0);
+    const uint8_t* bt = at + S0 + (r0 * k.nbp & 15);
+    auto x_of = [&](int row, int c) -> float {
+      if constexpr (KEPT) return kept8_number(ct[row * k.Cp + c]) * kept8_step(bt[row * k.nbp + c / kKeptBlock]);
+      else return to_f32(xt[row * C + c]);
+    };
+    // with d = x - mean and g' = dy w rstd:  a = mean_c(g'),  b = rstd^2 mean_c(g' d)
+    for (int u = warp; u < pl.rows * pl.segs; u += WARPS) {
+      const int row = u / pl.segs, seg = u % pl.segs;
+      const bool in = r0 + row < rows;
+      if (!in && pl.segs == 1) break;
+      const int c0 = min(C, seg * width), c1 = in ? min(C, c0 + width) : c0;
+      const float2 st = in ? *reinterpret_cast<const float2*>(stats + 2 * (r0 + row)) : make_float2(0.f, 0.f);
+      float sg = 0.f, sn = 0.f;
+      if (dx != nullptr) {
+        float gs[2] = {0.f, 0.f}, ns[2] = {0.f, 0.f};
+        int c = c0 + lane;
+        for (; c + 32 < c1; c += 64) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float gw = to_f32(gt[row * C + c + 32 * j]) * st.y * w[c + 32 * j];
+            gs[j] += gw;
+            ns[j] = fmaf(gw, x_of(row, c + 32 * j) - st.x, ns[j]);
+          }
+        }
+        if (c < c1) {
+          const float gw = to_f32(gt[row * C + c]) * st.y * w[c];
+          gs[0] += gw;
+          ns[0] = fmaf(gw, x_of(row, c) - st.x, ns[0]);
+        }
+        sg = join_segs(warp_sum(gs[0] + gs[1]), &parts[0][row * pl.segs], seg, pl.segs);
+        sn = join_segs(warp_sum(ns[0] + ns[1]), &parts[1][row * pl.segs], seg, pl.segs);
+      }
+      if (lane == 0 && seg == 0)
+        row_of[row] = make_float4(st.x, st.y, layer ? sg * inv_c : 0.f, sn * inv_c * st.y * st.y);
+    }
+    __syncthreads();
+    const int n = (int)count(r0);
+    for (int row = 0; row < n; ++row) {
+      const float4 q = row_of[row];
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int c = t + i * NT;
+        if (c >= C) continue;
+        const float g = to_f32(gt[row * C + c]), d = x_of(row, c) - q.x, gr = g * q.y;
+        aw[i] = fmaf(gr, d, aw[i]);
+        ab[i] += g;
+        // the product rounded as in phase 1, so that equal terms cancel
+        if (dx != nullptr) gt[row * C + c] = from_f32<T>(fmaf(-d, q.w, __fmul_rn(gr, w[c]) - q.z));
+      }
+    }
+    __syncthreads();
+    if (dx != nullptr) {
+      FlatRun<T>(dx, (long long)r0 * C, count(r0) * C).store(at);  // dx is aligned as dy is: the same offsets
+      __syncthreads();
+    }
+  }
+  copy_wait<0>();
+  if (part == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int c = t + i * NT;
+    if (c >= C) continue;
+    store_partial(aw[i], c, C, 0, vec.fp32, part, dw);
+    store_partial(ab[i], c, C, 1, vec.fp32, part, db);
   }
 }
 
@@ -1091,16 +1307,70 @@ void fwd_single(const FwdCall& f) {
 }
 
 template <typename T, int G, int UPT, int R>
-void fwd_flat(const FwdCall& f) {
+void fwd_group(const FwdCall& f) {
   using B = FlatBatch<T, G, UPT, R>;
-  constexpr int BYTES = flat_depth(G) * B::ROOM;
-  static_assert(BYTES * flat_ctas(G, R) <= kRingBudget, "the batches of an SM's CTAs do not fit its shared memory");
+  constexpr int BYTES = kGroupDepth * B::ROOM;
+  static_assert(BYTES * kGroupCtas <= kRingBudget, "the batches of an SM's CTAs do not fit its shared memory");
   const auto kernel = norm_fwd_flat_kernel<T, G, UPT, R>;
   static bool ready = false;
   if (!ready) ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) == cudaSuccess;
-  kernel<<<grid_for(f.a.rows, B::ROWS, flat_ctas(G, R)), B::NT, BYTES, f.s>>>((const T*)f.x.p, (uint32_t)f.a.rows, f.a.C,
+  kernel<<<grid_for(f.a.rows, B::ROWS, kGroupCtas), B::NT, BYTES, f.s>>>((const T*)f.x.p, (uint32_t)f.a.rows, f.a.C,
                                                                            f.vec(), f.a.eps, f.a.layer, (T*)f.y,
                                                                            f.stats, kept_of(f.k));
+}
+
+// Batches whose two stages and vectors fit half an SM's shared memory (two CTAs): as many rows as give 32 KB, a multiple of
+// the warps, or fewer where rows are long; then several warps share a row.  rows == 0: not even one row fits an SM.
+FlatPlan flat_plan(int C, int esize, int tensors, bool kept, int vectors, int warps) {
+  FlatPlan p{};
+  const long long Cp = (C + kKeptBlock - 1) / kKeptBlock * kKeptBlock, nbp = (Cp / kKeptBlock + 3) / 4 * 4;
+  const long long row = (long long)tensors * C * esize + (kept ? Cp + nbp : 0), fixed = (long long)vectors * C * 4 + 32;
+  auto fits = [&](long long rows, long long budget) {
+    return kFlatDepth * (rows * row + 96) + fixed + rows * 16 <= budget;
+  };
+  const long long half = kRingBudget / 2;
+  long long rows = 32 * 1024 / row / warps * warps;
+  if (rows > 256) rows = 256;
+  if (rows < warps || !fits(rows, half)) {
+    rows = warps;
+    while (rows > 1 && !fits(rows, half)) rows /= 2;
+    if (!fits(rows, kRingBudget)) return p;
+  }
+  p.rows = (int)rows;
+  p.segs = rows < warps ? (int)(warps / rows) : 1;
+  auto room = [](long long bytes) { return (uint32_t)((bytes + 30) / 16 * 16); };
+  p.room = room(rows * C * esize);
+  p.codes = kept ? room(rows * Cp) : 0;
+  p.scales = kept ? room(rows * nbp) : 0;
+  p.stage = tensors * p.room + p.codes + p.scales;
+  p.vectors = kFlatDepth * p.stage;
+  return p;
+}
+int flat_bytes(const FlatPlan& p, int C, int vectors) { return (int)(p.vectors + ((size_t)vectors * C + 4) * 4 + p.rows * 16); }
+
+template <typename K>
+void allow_smem(K kernel, int bytes, int& allowed) {
+  if (bytes > allowed && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess)
+    allowed = bytes;
+}
+
+template <typename T>
+bool fwd_flat(const FwdCall& f) {
+  const int C = f.a.C;
+  constexpr int R = sizeof(T) == 2 ? 4 : 2;  // batches of about 16 KB
+  if (C <= 64) return fwd_group<T, 8, 2, R>(f), true;
+  if (C <= 128) return fwd_group<T, 16, 2, R>(f), true;
+  if (C <= 256) return fwd_group<T, 32, 2, R>(f), true;
+  if (C <= 512) return fwd_group<T, 64, 2, R>(f), true;
+  if (C <= 1024) return fwd_group<T, 128, 2, R>(f), true;
+  const FlatPlan pl = flat_plan(f.a.C, sizeof(T), 1, false, 2, kThreads / 32);
+  if (pl.rows == 0) return false;
+  const int bytes = flat_bytes(pl, f.a.C, 2);
+  static int allowed = 48 * 1024;
+  allow_smem(norm_fwd_long_kernel<T>, bytes, allowed);
+  norm_fwd_long_kernel<T><<<grid_for(f.a.rows, pl.rows, 2), kThreads, bytes, f.s>>>(
+      (const T*)f.x.p, (uint32_t)f.a.rows, f.a.C, f.vec(), f.a.eps, f.a.layer, (T*)f.y, f.stats, kept_of(f.k), pl);
+  return true;
 }
 
 template <typename T, bool LAYER>
@@ -1125,18 +1395,7 @@ void fwd(const FwdCall& f) {
   const int C = f.a.C;
   if (C % 8 == 0 && C <= 16384 && rows_aligned16(f.x, f.a.fp32) && aligned16(f.a.w) && aligned16(f.a.b))
     return f.a.layer ? fwd_staged_any<T, true>(f) : fwd_staged_any<T, false>(f);
-  // batches of about 16 KB
-  constexpr int R = sizeof(T) == 2 ? 4 : 2;
-  if (contiguous_rows(f.x, C)) {
-    if (C <= 64) return fwd_flat<T, 8, 2, R>(f);
-    if (C <= 128) return fwd_flat<T, 16, 2, R>(f);
-    if (C <= 256) return fwd_flat<T, 32, 2, R>(f);
-    if (C <= 512) return fwd_flat<T, 64, 2, R>(f);
-    if (C <= 1024) return fwd_flat<T, 128, 2, R>(f);
-    if (C <= 2048) return fwd_flat<T, 256, 2, R>(f);
-    if (C <= 4096) return fwd_flat<T, 512, 2, 2>(f);
-    if (C <= 8192) return fwd_flat<T, 512, 4, sizeof(T) == 2 ? 2 : 1>(f);
-  }
+  if (contiguous_rows(f.x, C) && fwd_flat<T>(f)) return;
   if (C <= 256) return fwd_single<T, 32, 8, 2>(f);
   if (C <= 2048) return fwd_single<T, 256, 8, 2>(f);
   if (C <= 8192) return fwd_single<T, 512, 16, 1>(f);
@@ -1196,11 +1455,11 @@ void bwd_single(const BwdCall& b) {
 }
 
 template <typename T, int G, int UPT, int R, bool KEPT>
-void bwd_flat(const BwdCall& b) {
+void bwd_group(const BwdCall& b) {
   using B = FlatBatch<T, G, UPT, R>;
-  constexpr int BYTES = flat_depth(G) * (B::ROOM + (KEPT ? B::CODES + B::SCALES : B::ROOM));
-  static_assert(BYTES * flat_ctas(G, R) <= kRingBudget, "the batches of an SM's CTAs do not fit its shared memory");
-  const int grid = grid_for(b.a.rows, B::ROWS, flat_ctas(G, R));
+  constexpr int BYTES = kGroupDepth * (B::ROOM + (KEPT ? B::CODES + B::SCALES : B::ROOM));
+  static_assert(BYTES * kGroupCtas <= kRingBudget, "the batches of an SM's CTAs do not fit its shared memory");
+  const int grid = grid_for(b.a.rows, B::ROWS, kGroupCtas);
   if (b.parts != nullptr) {
     *b.parts = grid;
     return;
@@ -1211,6 +1470,39 @@ void bwd_flat(const BwdCall& b) {
   kernel<<<grid, B::NT, BYTES, b.s>>>((const T*)b.dy.p, (const T*)b.x.p, kept_of(b.k), (uint32_t)b.a.rows, b.a.C,
                                       b.vec(), b.a.layer, b.stats, (T*)b.dx, b.part, b.dw, b.db);
   b.finish(grid);
+}
+
+template <typename T, int NT, int E, bool KEPT>
+bool bwd_long(const BwdCall& b) {
+  const FlatPlan pl = flat_plan(b.a.C, sizeof(T), KEPT ? 1 : 2, KEPT, 1, NT / 32);
+  if (pl.rows == 0) return false;
+  const int grid = grid_for(b.a.rows, pl.rows, NT == 256 ? 2 : 1);
+  if (b.parts != nullptr) {
+    *b.parts = grid;
+    return true;
+  }
+  const int bytes = flat_bytes(pl, b.a.C, 1);
+  static int allowed = 48 * 1024;
+  allow_smem(norm_bwd_long_kernel<T, NT, E, KEPT>, bytes, allowed);
+  norm_bwd_long_kernel<T, NT, E, KEPT><<<grid, NT, bytes, b.s>>>(
+      (const T*)b.dy.p, (const T*)b.x.p, kept_of(b.k), (uint32_t)b.a.rows, b.a.C, b.vec(), b.a.layer, b.stats, (T*)b.dx,
+      b.part, b.dw, b.db, pl);
+  b.finish(grid);
+  return true;
+}
+
+template <typename T, bool KEPT>
+bool bwd_flat_any(const BwdCall& b) {
+  const int C = b.a.C;
+  if (C <= 64) return bwd_group<T, 8, 2, 2, KEPT>(b), true;
+  if (C <= 128) return bwd_group<T, 16, 2, 2, KEPT>(b), true;
+  if (C <= 256) return bwd_group<T, 32, 2, 2, KEPT>(b), true;
+  if (C <= 512) return bwd_group<T, 64, 2, 2, KEPT>(b), true;
+  if (C <= 1024) return bwd_group<T, 128, 2, 2, KEPT>(b), true;
+  if (C <= 2048) return bwd_long<T, 256, 8, KEPT>(b);
+  if (C <= 4096) return bwd_long<T, 256, 16, KEPT>(b);
+  if (C <= 8192) return bwd_long<T, 512, 16, KEPT>(b);
+  return false;
 }
 
 template <typename T>
@@ -1255,17 +1547,7 @@ void bwd(const BwdCall& b) {
   const bool fp32 = sizeof(T) == 4;
   if (C % 8 == 0 && C <= 16384 && rows_aligned16(b.dy, fp32) && (KEPT || rows_aligned16(b.x, fp32)) && aligned16(b.a.w))
     return b.a.layer ? bwd_staged_any<T, true, KEPT>(b) : bwd_staged_any<T, false, KEPT>(b);
-  constexpr int R = 2;
-  if (contiguous_rows(b.dy, C) && (KEPT || contiguous_rows(b.x, C))) {
-    if (C <= 64) return bwd_flat<T, 8, 2, R, KEPT>(b);
-    if (C <= 128) return bwd_flat<T, 16, 2, R, KEPT>(b);
-    if (C <= 256) return bwd_flat<T, 32, 2, R, KEPT>(b);
-    if (C <= 512) return bwd_flat<T, 64, 2, R, KEPT>(b);
-    if (C <= 1024) return bwd_flat<T, 128, 2, R, KEPT>(b);
-    if (C <= 2048) return bwd_flat<T, 256, 2, R, KEPT>(b);
-    if (C <= 4096) return bwd_flat<T, 512, 2, R, KEPT>(b);
-    if (C <= 8192) return bwd_flat<T, 512, 4, 1, KEPT>(b);
-  }
+  if (contiguous_rows(b.dy, C) && (KEPT || contiguous_rows(b.x, C)) && bwd_flat_any<T, KEPT>(b)) return;
   if (C <= 256) return bwd_single<T, 32, 8, 2, KEPT>(b);
   if (C <= 2048) return bwd_single<T, 256, 8, 2, KEPT>(b);
   if (C <= 8192) return bwd_single<T, 1024, 8, 1, KEPT>(b);
