@@ -305,26 +305,22 @@ bool is_operand(const torch::Tensor& t) {
          reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
-// `t` as a GEMM operand: itself, or a copy with rows of C rounded up to 8 (zeros past C).
-torch::Tensor operand(const torch::Tensor& t) {
-  const int64_t C = t.size(1);
-  if (is_operand(t)) return t;
+// A zero-padded copy of bf16 rows.
+torch::Tensor padded(const torch::Tensor& t, int64_t rows, int64_t width) {
   const RowsOf r = rows_of(t, "operand");
-  auto out = torch::empty({t.size(0), up8(C)}, t.options());
-  launch_pad_rows(r.a, r.rows, r.C, out.data_ptr(), out.size(1), stream());
+  auto out = torch::empty({rows, width}, t.options());
+  launch_pad_rows(r.a, r.rows, r.C, out.data_ptr(), rows, width, stream());
   check_launch(nullptr, "pad_rows");
   return out;
 }
 
+// `t` as a GEMM operand: itself, or a copy with rows of C rounded up to 8 (zeros past C).
+torch::Tensor operand(const torch::Tensor& t) { return is_operand(t) ? t : padded(t, t.size(0), up8(t.size(1))); }
+
 // The weight as an operand: also its row count a multiple of 8.
 torch::Tensor weight_operand(const torch::Tensor& w_) {
   const torch::Tensor w = w_.scalar_type() == torch::kBFloat16 ? w_ : w_.to(torch::kBFloat16);
-  if (w.size(0) % 8 == 0) return operand(w);
-  const RowsOf r = rows_of(w, "weight");
-  auto out = torch::empty({up8(w.size(0)), up8(w.size(1))}, w.options());
-  launch_pad_rows(r.a, r.rows, r.C, out.data_ptr(), out.size(1), stream());
-  out.narrow(0, w.size(0), out.size(0) - w.size(0)).zero_();
-  return out;
+  return w.size(0) % 8 == 0 && is_operand(w) ? w : padded(w, up8(w.size(0)), up8(w.size(1)));
 }
 
 // dw (+)= g[row0 : row0 + rows]^T x[: rows]; g and x as operands.
@@ -385,8 +381,8 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     if (rows > 0) {
       OptTensor bias;
       if (b.has_value()) {
-        bias = b->to(torch::kBFloat16).contiguous();
-        if (N % 8 != 0) bias = torch::constant_pad_nd(*bias, {0, up8(N) - N});
+        const torch::Tensor bf = b->scalar_type() == torch::kBFloat16 ? *b : b->to(torch::kBFloat16);
+        bias = N % 8 == 0 ? bf.contiguous() : padded(bf.unsqueeze(0), 1, up8(N)).view({up8(N)});
       }
       gemm(xp, weight_operand(w), y, true, true, bias, c10::nullopt, false);
     }
@@ -395,7 +391,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
       ctx->saved_data["shape"] = x.sizes().vec();
       ctx->saved_data["b_type"] = b.has_value() ? (int64_t)b->scalar_type() : (int64_t)-1;
     }
-    return y.narrow(1, 0, N).view(shape);
+    return N % 8 == 0 ? y.view(shape) : y.narrow(1, 0, N).view(shape);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -412,7 +408,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     if (need_dx) {
       auto out = torch::empty({rows, up8(K)}, gy.options());
       if (rows > 0) gemm(gp, weight_operand(w), out, true, false, c10::nullopt, c10::nullopt, false);
-      dx = out.narrow(1, 0, K).view(ctx->saved_data["shape"].toIntVector());
+      dx = (K % 8 == 0 ? out : out.narrow(1, 0, K)).view(ctx->saved_data["shape"].toIntVector());
     }
     if (need_dw) dw = weight_grad8(gp, N, codes, scales, K, w.scalar_type() == torch::kFloat32);
     if (need_db) {

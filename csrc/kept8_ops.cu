@@ -117,18 +117,18 @@ __global__ void __launch_bounds__(kThreads) keep8_kernel(RowView x, Units un, Ke
   }
 }
 
-// out [rows, ld] = x [rows, C] with zeros past C, eight elements a thread (ld % 8 == 0).
-__global__ void __launch_bounds__(kThreads) pad_rows_kernel(RowView x, Units un, int C,
+// out [out_rows, ld] = x [rows, C] with zeros past C and past the rows, eight elements a thread (ld % 8 == 0).
+__global__ void __launch_bounds__(kThreads) pad_rows_kernel(RowView x, Units un, uint32_t rows, int C,
                                                             __nv_bfloat16* __restrict__ out, long long ld) {
   const uint32_t u = blockIdx.x * kThreads + threadIdx.x;
   if (u >= un.total) return;
   uint32_t row;
   int c;
   unit_at<8>(un, u, row, c);
-  const __nv_bfloat16* p = row_ptr<__nv_bfloat16>(x, row);
+  const __nv_bfloat16* p = row_ptr<__nv_bfloat16>(x, row < rows ? row : 0);
   float v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = c + i < C ? to_f32(p[c + i]) : 0.f;
+  for (int i = 0; i < 8; ++i) v[i] = row < rows && c + i < C ? to_f32(p[c + i]) : 0.f;
   store8(out + (long long)row * ld + c, v);
 }
 
@@ -728,16 +728,11 @@ void launch_swiglu_bwd(const RowsArg& dh, long long rows, bool fp32, const Kept8
 #undef CALL
 }
 
-void launch_pad_rows(const RowsArg& x, long long rows, int C, void* out, long long ld, cudaStream_t s) {
-  const uint32_t per_row = (uint32_t)(ld / 8);
-  const long long chunk = kMaxUnits / per_row;
-  for (long long r0 = 0; r0 < rows; r0 += chunk) {
-    Units un;
-    un.row0 = (uint32_t)r0;
-    un.per_row = FastDiv(per_row);
-    un.total = (uint32_t)((rows - r0 < chunk ? rows - r0 : chunk) * per_row);
-    pad_rows_kernel<<<(un.total + kThreads - 1) / kThreads, kThreads, 0, s>>>(view_of(x), un, C, (__nv_bfloat16*)out, ld);
-  }
+void launch_pad_rows(const RowsArg& x, long long rows, int C, void* out, long long out_rows, long long ld,
+                     cudaStream_t s) {
+  over_rows<8, 1>(out_rows, (int)ld, [&](const Units& un, uint32_t grid) {
+    pad_rows_kernel<<<grid, kThreads, 0, s>>>(view_of(x), un, (uint32_t)rows, C, (__nv_bfloat16*)out, ld);
+  });
 }
 
 // One chunk (and one launch) up to 1024 rows; beyond, as many as fill the GPU about four times with chunks of at

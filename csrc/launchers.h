@@ -44,8 +44,9 @@ struct Kept8Buf {
 // copy (bf16 x only, may be null): x itself with row stride ld, ld / 8 whole, zeros past C.
 void launch_keep8(const RowsArg& x, long long rows, bool fp32, const Kept8Buf& k, void* copy, long long ld,
                   cudaStream_t s);
-// out [rows, ld] bf16 = x [rows, C], zeros past C (ld = C rounded up to 8).
-void launch_pad_rows(const RowsArg& x, long long rows, int C, void* out, long long ld, cudaStream_t s);
+// out [out_rows, ld] bf16 = x [rows, C], zeros past C and past the rows (ld a multiple of 8).
+void launch_pad_rows(const RowsArg& x, long long rows, int C, void* out, long long out_rows, long long ld,
+                     cudaStream_t s);
 // Rows row0 .. row0 + rows of `k` into out (row stride ld): `cols` columns, C or more (zeros past C) and at most
 // the codes' padded width.
 void launch_restore8(const Kept8Buf& k, long long row0, long long rows, bool fp32, void* out, long long ld, int cols,
