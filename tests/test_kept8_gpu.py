@@ -168,6 +168,15 @@ def test_norm_of_narrow_rows(C, dtype, layer, kept):
 
 
 @DTYPES
+@KINDS
+@KEPT
+@pytest.mark.parametrize("rows,C", [(4001, 264), (1000, 384), (2570, 520), (64, 768), (90, 1032), (1601, 1536), (700, 2056),
+                                    (333, 4104), (310, 6144)])
+def test_norm_between_powers_of_two(rows, C, dtype, layer, kept):
+    norm_case((rows, C), dtype, layer, kept, seed=C)
+
+
+@DTYPES
 @KEPT
 @pytest.mark.parametrize("rows,C", [(20011, 33), (1, 257), (9000, 511), (1300, 1023), (700, 2047), (301, 3001), (611, 4097),
                                     (150, 8191), (12, 8193)])
