@@ -187,18 +187,8 @@ __device__ __forceinline__ uint32_t pack4_low_bytes(uint32_t a, uint32_t b, uint
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-template <int V>
-__device__ __forceinline__ void kept8_store_codes(int8_t* p, const float (&v)[V], uint32_t b) {
-  const float inv = kept8_inv_step(b);
-  if constexpr (V == 1) {
-    *p = (int8_t)(kept8_code(v[0], inv) & 0xffu);
-  } else {
-    uint32_t c[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = kept8_code(v[i], inv);
-    *reinterpret_cast<uint2*>(p) =
-        make_uint2(pack4_low_bytes(c[0], c[1], c[2], c[3]), pack4_low_bytes(c[4], c[5], c[6], c[7]));
-  }
+__device__ __forceinline__ void kept8_store_code(int8_t* p, float v, uint32_t b) {
+  *p = (int8_t)(kept8_code(v, kept8_inv_step(b)) & 0xffu);
 }
 
 // Eight codes as numbers.
@@ -226,14 +216,6 @@ __device__ __forceinline__ void kept8_values(uint2 w, float step, float (&v)[8])
   kept8_values(w, step, p);
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[2 * i] = p[i].x, v[2 * i + 1] = p[i].y;
-}
-
-// V codes from `p` times the step of scale byte b.
-template <int V>
-__device__ __forceinline__ void kept8_load(const int8_t* p, uint32_t b, float (&v)[V]) {
-  const float step = kept8_step(b);
-  if constexpr (V == 1) v[0] = kept8_number(*p) * step;
-  else kept8_values(*reinterpret_cast<const uint2*>(p), step, v);
 }
 
 // Scale byte and codes of a fragment whose block is held by four neighbouring lanes; every lane of the

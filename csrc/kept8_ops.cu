@@ -80,7 +80,7 @@ __device__ __forceinline__ void keep_fragment(const Kept8Out& o, uint32_t row, i
   } else {
     const float v[1] = {x.f};
     b = kept8_byte(kept8_amax<1>(v));
-    if (act) kept8_store_codes<1>(at, v, b);
+    if (act) kept8_store_code(at, x.f, b);
   }
   if (act && c % kKeptBlock == 0) kept8_store_byte(o.scales + (long long)row * o.nbp, c / kKeptBlock, o.nb, o.nbp, b);
 }
@@ -93,6 +93,9 @@ __device__ __forceinline__ void kept_pairs(const Kept8Out& k, uint32_t row, int 
   else v[0] = make_float2(kept8_number(*p) * step, 0.f);
 }
 
+// A block's scale is the exponent of its largest |x|: four lanes agree on it by two exchanges, so x is read once.  Bound by
+// DRAM (3.03 B an element in bf16, twice as many reads as writes): 110576 x 4096 240 us (5.7 TB/s), fp32 330 us
+// (6.9 TB/s); odd widths through tiles 200001 x 1001 bf16 144 us (4.2 TB/s).  U = 4 fragments in flight a thread hide the latency.
 // `copy`, when given, also gets x itself with rows of `ld` elements and zeros past C: the operand that a
 // GEMM can read of rows that are not 16-byte aligned.
 template <typename T, int V, int U>
@@ -132,6 +135,8 @@ __global__ void __launch_bounds__(kThreads) pad_rows_kernel(RowView x, Units un,
   store8(out + (long long)row * ld + c, v);
 }
 
+// code * step, exact in bf16, so one rounding-free store.  Bound by DRAM: 110576 x 4096 to bf16 232 us (5.9 TB/s), to fp32 430
+// us (5.3 TB/s, where stores are four fifths of the bytes).
 template <typename T, int V, int U>
 __global__ void __launch_bounds__(kThreads) restore8_kernel(Units un, Kept8Out k8, T* __restrict__ out, long long ld) {
   const uint32_t u0 = blockIdx.x * (kThreads * U) + threadIdx.x;
@@ -159,7 +164,8 @@ __device__ __forceinline__ float sigmoid_fast(float g) {
   return s;
 }
 
-// h = silu(g) * u; both inputs' codes are written beside it.
+// h = silu(g) * u; both inputs' codes are written beside it.  Bound by DRAM: 16384 x 16384 bf16 361 us (6.0 TB/s), the codes in
+// packed pairs and the sigmoid in two hardware instructions to keep issue below it; 60000 x 1001 126 us (3.9 TB/s, tiles).
 template <typename T, int V, int U>
 __global__ void __launch_bounds__(kThreads) swiglu_fwd_kernel(RowView gate, RowView value, Units un, Kept8Out og,
                                                               Kept8Out ov, T* __restrict__ h) {
@@ -198,7 +204,8 @@ __global__ void __launch_bounds__(kThreads) swiglu_fwd_kernel(RowView gate, RowV
 }
 
 // dg = dh u s (1 + g (1 - s)),  du = dh g s  with s = sigmoid(g) and g, u read from their codes;
-// h, when asked for, is silu(g) u of the same values (the input of the projection that follows).
+// h, when asked for, is silu(g) u of the same values (the input of the projection that follows).  Bound by DRAM: 16384 x
+// 16384 bf16 322 us without h (6.7 TB/s); 60000 x 1001 125 us (3.9 TB/s, tiles).
 template <typename T, int V, int U>
 __global__ void __launch_bounds__(kThreads) swiglu_bwd_kernel(RowView dh, Kept8Out kg, Kept8Out kv, Units un,
                                                               T* __restrict__ dgate, T* __restrict__ dvalue,
@@ -238,7 +245,7 @@ __global__ void __launch_bounds__(kThreads) swiglu_bwd_kernel(RowView dh, Kept8O
 // ---------------------------------------------------------------- flat form
 // A tile is 16 KB of whole rows, or of one row when that is longer.  Its fragments are (row, V columns) over rows padded
 // to whole blocks, 32 / V lanes to a block.  V = 8 for bf16, where the kernels are bound by instructions: keep8 of 200001 x
-// 1001 took 242 us with 4 columns and 8 KB tiles, 190 with 8, 172 with the packed encoding, 156 with 16 KB tiles (3.9 TB/s).
+// 1001 took 242 us with 4 columns and 8 KB tiles, 190 with 8, 172 with the packed encoding, 144 with 16 KB tiles whose ends are copied in parallel (4.2 TB/s).
 // V = 4 for fp32, where 8 would read shared memory at half the rate.
 constexpr int flat_v(bool fp32) { return fp32 ? 4 : 8; }
 constexpr int flat_size(bool fp32) { return fp32 ? 4096 : 8192; }  // 16 KB
@@ -309,25 +316,18 @@ __device__ __forceinline__ Frag<__nv_bfloat16> flat_frag8(const uint8_t* smem, c
   return x;
 }
 
-// Scale and codes of a fragment; all lanes of the warp take part, `act` lanes store.
-template <int V>
-__device__ __forceinline__ void flat_keep(const Kept8Out& o, uint32_t row, int c, bool act, const float (&v)[V]) {
+// Scale and codes of four columns; all lanes of the warp take part, `act` lanes store.
+__device__ __forceinline__ void flat_keep(const Kept8Out& o, uint32_t row, int c, bool act, const float (&v)[4]) {
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
 #pragma unroll
-  for (int d = 1; d < kKeptBlock / V; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  for (int d = 1; d < kKeptBlock / 4; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
   const uint32_t b = kept8_byte(m);
   if (!act) return;
   const float inv = kept8_inv_step(b);
-  uint32_t w[V / 4];
-#pragma unroll
-  for (int i = 0; i < V / 4; ++i)
-    w[i] = pack4_low_bytes(kept8_code(v[4 * i], inv), kept8_code(v[4 * i + 1], inv), kept8_code(v[4 * i + 2], inv),
-                           kept8_code(v[4 * i + 3], inv));
-  int8_t* at = o.codes + (long long)row * o.Cp + c;
-  if constexpr (V == 8) *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
-  else *reinterpret_cast<uint32_t*>(at) = w[0];
+  *reinterpret_cast<uint32_t*>(o.codes + (long long)row * o.Cp + c) =
+      pack4_low_bytes(kept8_code(v[0], inv), kept8_code(v[1], inv), kept8_code(v[2], inv), kept8_code(v[3], inv));
   if (c % kKeptBlock == 0) kept8_store_byte(o.scales + (long long)row * o.nbp, c / kKeptBlock, o.nb, o.nbp, b);
 }
 

@@ -13,7 +13,7 @@
 // registers, and one partial row of dw / db per CTA goes to scratch, which a second kernel adds up in order (no
 // atomics: the same bits every time).  Four forms:
 //   staged   (C % 8 == 0, 16-byte aligned rows, C <= 16384)  8-column fragments through rings in shared memory
-//   flat     (contiguous rows of other widths, C <= 8192)    batches of rows as runs of bytes (flat.cuh)
+//   flat     (contiguous rows of other widths, C <= 8192)    batches of rows as runs of bytes (flat.cuh): groups, or warps (long rows)
 //   single   (other views, C <= 8192)                        one column at a time, straight from memory
 //   wide     (wider rows)                                    CTA per row, the row swept from memory
 // Groups of up to a warp reduce by shuffles, larger ones through shared memory.
@@ -182,7 +182,8 @@ __device__ __forceinline__ void zero_ring(uint8_t* ring, int bytes) {
 }
 
 // R rows a group a turn.  x is read once: into the ring, from there into registers, which the mean, the centred squares, the
-// codes and y all use.
+// codes and y all use.  Bound by DRAM: layer norm of 94960 x 4096 bf16 255 us (6.1 TB/s), kept 366 us (5.3 TB/s: the codes'
+// arithmetic shares the issue slots); 16384 x 32 x 128 RMS 52 us (5.2 TB/s).
 template <typename T, int G, int UPT, int R, int DEPTH, int CTAS, bool LAYER>
 __global__ void __launch_bounds__(threads_of(G), CTAS)
     norm_fwd_staged_kernel(RowView x, uint32_t rows, int C, Vectors vec, float eps, T* __restrict__ y,
@@ -327,7 +328,9 @@ __device__ __forceinline__ void store_partial(float v, int c, int C, int which, 
 }
 
 // One row a group a turn.  Between the sums and dx a thread holds its g' and x - mean as fp32 (UPT = 2: 32
-// registers); with more columns, where dw and db take the registers, it reads the ring a second time.
+// registers); with more columns, where dw and db take the registers, it reads the ring a second time.  Bound by DRAM: layer
+// norm of 94960 x 4096 bf16 390 us (6.0 TB/s), from the codes 389 us (5.0 TB/s; decoding shares the issue slots; three
+// CTAs an SM that hold nothing took 144 us for 24414 rows against 119).
 template <typename T, int G, int UPT, int DEPTH, int CTAS, bool LAYER, bool KEPT>
 __global__ void __launch_bounds__(threads_of(G), CTAS)
     norm_bwd_staged_kernel(RowView dy, RowView x, Kept k, uint32_t rows, int C, Vectors vec,
@@ -498,10 +501,14 @@ __global__ void __launch_bounds__(threads_of(G), CTAS)
 }
 
 // ---------------------------------------------------------------- flat form
-// Rows of up to 1024 columns.  A batch is GROUPS * R neighbouring rows, one run of bytes; the next two or three arrive while one is worked on (one
-// ahead left the kernel waiting for memory at 35 % of its bandwidth).  Fragment i of thread t are the 4 columns from 4 (t + i G) on: eight lanes hold a block of
-// the codes.  Results take the place of the input and leave as one run.
-constexpr int kGroupCtas = 2;
+// A batch is GROUPS * R neighbouring rows, one run of bytes; the next two arrive while one is worked on (with one, the kernel
+// waited for memory at 35 % of its bandwidth).  Fragment i of thread t are the 4 columns from 4 (t + i G) on: eight lanes
+// hold a block of the codes.  Results take the place of the input and leave as one run.  What bounds it is instruction
+// issue: single elements are read, converted and masked (48 instructions an element in the forward of width 631), so
+// bf16 groups are sized for few idle lanes: 100 M elements, layer norm, kept forward / kept backward, two fragments of
+// twice the threads and then three a thread: width 333 269 / 250 and 210 / 182 us, 631 268 / 272 and 215 / 192, 77 291 / 249
+// and 213 / 191.
+constexpr int group_ctas(int G) { return G > kThreads ? 1 : 2; }
 constexpr int kGroupDepth = 3;
 
 template <typename T, int G, int UPT, int R>
@@ -526,7 +533,7 @@ __device__ __forceinline__ void write4(T* p, int n, const float (&v)[4]) {
 }
 
 template <typename T, int G, int UPT, int R>
-__global__ void __launch_bounds__(threads_of(G), kGroupCtas)
+__global__ void __launch_bounds__(threads_of(G), group_ctas(G))
     norm_fwd_flat_kernel(const T* x, uint32_t rows, int C, Vectors vec, float eps, bool layer, T* __restrict__ y,
                          float* __restrict__ stats, Kept k) {
   using B = FlatBatch<T, G, UPT, R>;
@@ -628,7 +635,7 @@ __global__ void __launch_bounds__(threads_of(G), kGroupCtas)
 }
 
 template <typename T, int G, int UPT, int R, bool KEPT>
-__global__ void __launch_bounds__(threads_of(G), kGroupCtas)
+__global__ void __launch_bounds__(threads_of(G), group_ctas(G))
     norm_bwd_flat_kernel(const T* dy, const T* x, Kept k, uint32_t rows, int C, Vectors vec, bool layer,
                          const float* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, void* dw,
                          void* db) {
@@ -757,9 +764,10 @@ __global__ void __launch_bounds__(threads_of(G), kGroupCtas)
 // ---------------------------------------------------------------- flat form, long rows
 // Row sums are taken by whole warps, a row each (or `segs` warps a row where few rows fit): no barrier and no idle threads
 // per row.  Lanes read neighbouring columns, so odd widths cost no bank conflicts, and a warp's 32 columns are one block of
-// the codes.  Measured against the groups above, which hold a row in registers and reduce with a barrier: 40000 x 2169 bf16
-// kept forward 540 / 262 us, backward 601 / 327; 40000 x 1501 167 / 178 and 212 / 190; 100000 x 1001 198 / 325 and 251 / 287; so
-// rows of up to 1024 columns take the groups.
+// the codes; but each element is read from shared memory once a pass instead of being held.  For widths where groups do
+// not fit, or leave too much idle: fp32 1025 to 1536 and past 2048, bf16 past 6144.  100 M bf16 elements, kept forward / backward,
+// this form and then groups: width 1501 314 / 261 and 208 / 179 us, 2901 328 / 307 and 207 / 186, 5001 329 / 399 and 255 / 230; 50 M fp32:
+// 1101 171 / 186 and 203 / 187, 2047 185 / 179 and 132 / 139.
 constexpr int kFlatDepth = 2;
 struct FlatPlan {
   int rows, segs;          // rows of a batch; warps a row
@@ -847,7 +855,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const float v[1] = {c < c1 ? to_f32(xr[c]) : 0.f};
         if (k.codes != nullptr) {
           const uint32_t sb = kept8_byte(kept8_amax<1>(v));
-          kept8_store_codes<1>(codes + c, v, sb);
+          kept8_store_code(codes + c, v[0], sb);
           if (lane == 0) kept8_store_byte(scales, cb / kKeptBlock, k.nb, k.nbp, sb);
         }
         if (c < c1) xr[c] = from_f32<T>(fmaf((v[0] - mean) * rstd, w[c], b[c]));
@@ -1031,7 +1039,7 @@ __global__ void __launch_bounds__(threads_of(G), single_ctas(G))
           const float one[1] = {v[q][i]};
           const uint32_t sb = kept8_byte(kept8_amax<1>(one));
           if (in) {
-            kept8_store_codes<1>(codes + c, one, sb);
+            kept8_store_code(codes + c, one[0], sb);
             if (c % kKeptBlock == 0) kept8_store_byte(k.scales + (long long)r * k.nbp, c / kKeptBlock, k.nb, k.nbp, sb);
           }
         }
@@ -1175,7 +1183,7 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_wide_kernel(RowView x, uint
       float v[1] = {c < C ? to_f32(xr[c]) : 0.f};
       if (k.codes != nullptr) {  // Cp % 32 == 0: warps stay whole
         const uint32_t sb = kept8_byte(kept8_amax<1>(v));
-        kept8_store_codes<1>(k.codes + (long long)r * k.Cp + c, v, sb);
+        kept8_store_code(k.codes + (long long)r * k.Cp + c, v[0], sb);
         if (c % kKeptBlock == 0) kept8_store_byte(k.scales + (long long)r * k.nbp, c / kKeptBlock, k.nb, k.nbp, sb);
       }
       if (c < C) yr[c] = from_f32<T>((v[0] - mean) * rstd * vec_at(vec.w, vec.fp32, c, 1.f) + vec_at(vec.b, vec.fp32, c, 0.f));
@@ -1310,11 +1318,11 @@ template <typename T, int G, int UPT, int R>
 void fwd_group(const FwdCall& f) {
   using B = FlatBatch<T, G, UPT, R>;
   constexpr int BYTES = kGroupDepth * B::ROOM;
-  static_assert(BYTES * kGroupCtas <= kRingBudget, "the batches of an SM's CTAs do not fit its shared memory");
+  static_assert(BYTES * group_ctas(G) <= kRingBudget, "the batches of an SM's CTAs do not fit its shared memory");
   const auto kernel = norm_fwd_flat_kernel<T, G, UPT, R>;
   static bool ready = false;
   if (!ready) ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) == cudaSuccess;
-  kernel<<<grid_for(f.a.rows, B::ROWS, kGroupCtas), B::NT, BYTES, f.s>>>((const T*)f.x.p, (uint32_t)f.a.rows, f.a.C,
+  kernel<<<grid_for(f.a.rows, B::ROWS, group_ctas(G)), B::NT, BYTES, f.s>>>((const T*)f.x.p, (uint32_t)f.a.rows, f.a.C,
                                                                            f.vec(), f.a.eps, f.a.layer, (T*)f.y,
                                                                            f.stats, kept_of(f.k));
 }
@@ -1357,12 +1365,27 @@ void allow_smem(K kernel, int bytes, int& allowed) {
 template <typename T>
 bool fwd_flat(const FwdCall& f) {
   const int C = f.a.C;
-  constexpr int R = sizeof(T) == 2 ? 4 : 2;  // batches of about 16 KB
+  constexpr bool B16 = sizeof(T) == 2;
+  constexpr int R = B16 ? 4 : 2;  // batches of about 16 KB
   if (C <= 64) return fwd_group<T, 8, 2, R>(f), true;
-  if (C <= 128) return fwd_group<T, 16, 2, R>(f), true;
-  if (C <= 256) return fwd_group<T, 32, 2, R>(f), true;
-  if (C <= 512) return fwd_group<T, 64, 2, R>(f), true;
-  if (C <= 1024) return fwd_group<T, 128, 2, R>(f), true;
+#define GROUP(G) return fwd_group<T, G, 2, R>(f), true
+#define THIRDS(G) if constexpr (B16) if (C <= G * 12) return fwd_group<T, G, 3, 2>(f), true
+  if (C <= 64) GROUP(8);
+  THIRDS(8);
+  if (C <= 128) GROUP(16);
+  THIRDS(16);
+  if (C <= 256) GROUP(32);
+  THIRDS(32);
+  if (C <= 512) GROUP(64);
+  THIRDS(64);
+  if (C <= 1024) GROUP(128);
+  THIRDS(128);
+  if (C <= 2048 && (B16 || C > 1536)) GROUP(256);
+  THIRDS(256);
+  if constexpr (B16) if (C <= 4096) GROUP(512);
+  THIRDS(512);
+#undef THIRDS
+#undef GROUP
   const FlatPlan pl = flat_plan(f.a.C, sizeof(T), 1, false, 2, kThreads / 32);
   if (pl.rows == 0) return false;
   const int bytes = flat_bytes(pl, f.a.C, 2);
@@ -1383,7 +1406,7 @@ void fwd_staged_any(const FwdCall& f) {
   constexpr bool B16 = sizeof(T) == 2;
   constexpr int R = B16 ? 2 : 1, CTAS = B16 && LAYER ? 2 : 3, DEPTH = CTAS == 2 ? 6 : 4;
 #define STAGED(G) return fwd_staged<T, G, 2, R, DEPTH, CTAS, LAYER>(f)
-#define THIRDS(G) if (B16 && C <= G * 24) return fwd_staged<T, G, B16 ? 3 : 2, 1, B16 ? 8 : DEPTH, 2, LAYER>(f)
+#define THIRDS(G) if constexpr (B16) if (C <= G * 24) return fwd_staged<T, G, 3, 1, 8, 2, LAYER>(f)
   if (C <= 64) STAGED(4);
   if (C <= 128) STAGED(8);
   if (C <= 256) STAGED(16);
@@ -1470,8 +1493,8 @@ template <typename T, int G, int UPT, int R, bool KEPT>
 void bwd_group(const BwdCall& b) {
   using B = FlatBatch<T, G, UPT, R>;
   constexpr int BYTES = kGroupDepth * (B::ROOM + (KEPT ? B::CODES + B::SCALES : B::ROOM));
-  static_assert(BYTES * kGroupCtas <= kRingBudget, "the batches of an SM's CTAs do not fit its shared memory");
-  const int grid = grid_for(b.a.rows, B::ROWS, kGroupCtas);
+  static_assert(BYTES * group_ctas(G) <= kRingBudget, "the batches of an SM's CTAs do not fit its shared memory");
+  const int grid = grid_for(b.a.rows, B::ROWS, group_ctas(G));
   if (b.parts != nullptr) {
     *b.parts = grid;
     return;
@@ -1506,13 +1529,29 @@ bool bwd_long(const BwdCall& b) {
 template <typename T, bool KEPT>
 bool bwd_flat_any(const BwdCall& b) {
   const int C = b.a.C;
-  if (C <= 64) return bwd_group<T, 8, 2, 2, KEPT>(b), true;
-  if (C <= 128) return bwd_group<T, 16, 2, 2, KEPT>(b), true;
-  if (C <= 256) return bwd_group<T, 32, 2, 2, KEPT>(b), true;
-  if (C <= 512) return bwd_group<T, 64, 2, 2, KEPT>(b), true;
-  if (C <= 1024) return bwd_group<T, 128, 2, 2, KEPT>(b), true;
-  if (C <= 2048) return bwd_long<T, 256, 8, KEPT>(b);
-  if (C <= 4096) return bwd_long<T, 256, 16, KEPT>(b);
+  constexpr bool B16 = sizeof(T) == 2;
+#define GROUP(G) return bwd_group<T, G, 2, 2, KEPT>(b), true
+#define THIRDS(G) if constexpr (B16) if (C <= G * 12) return bwd_group<T, G, 3, 2, KEPT>(b), true
+  if (C <= 64) GROUP(8);
+  THIRDS(8);
+  if (C <= 128) GROUP(16);
+  THIRDS(16);
+  if (C <= 256) GROUP(32);
+  THIRDS(32);
+  if (C <= 512) GROUP(64);
+  THIRDS(64);
+  if (C <= 1024) GROUP(128);
+  THIRDS(128);
+  if (C <= 2048 && (B16 || C > 1536)) GROUP(256);
+  THIRDS(256);
+  if constexpr (B16) if (C <= 4096) GROUP(512);
+  THIRDS(512);
+#undef THIRDS
+#undef GROUP
+  if constexpr (!B16) {
+    if (C <= 1536) return bwd_long<T, 256, 6, KEPT>(b);
+    if (C <= 4096) return bwd_long<T, 256, 16, KEPT>(b);
+  }
   if (C <= 8192) return bwd_long<T, 512, 16, KEPT>(b);
   return false;
 }
@@ -1542,7 +1581,7 @@ void bwd_staged_any(const BwdCall& b) {
   constexpr bool B16 = sizeof(T) == 2;
   constexpr int DEPTH = B16 ? 6 : 3;
 #define STAGED(G) return bwd_staged<T, G, 2, DEPTH, 2, LAYER, KEPT>(b)
-#define THIRDS(G) if (B16 && C <= G * 24) return bwd_staged<T, G, B16 ? 3 : 2, !B16 ? DEPTH : KEPT ? 5 : 4, 2, LAYER, KEPT>(b)
+#define THIRDS(G) if constexpr (B16) if (C <= G * 24) return bwd_staged<T, G, 3, KEPT ? 5 : 4, 2, LAYER, KEPT>(b)
   if (C <= 64) STAGED(4);
   if (C <= 128) STAGED(8);
   if (C <= 256) STAGED(16);

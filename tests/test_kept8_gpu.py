@@ -177,6 +177,15 @@ def test_norm_between_powers_of_two(rows, C, dtype, layer, kept):
 
 
 @DTYPES
+@KINDS
+@KEPT
+@pytest.mark.parametrize("rows,C", [(5001, 77), (1201, 191), (1000, 379), (900, 767), (611, 1101), (307, 1535), (301, 1601),
+                                    (401, 2901), (310, 3501), (300, 6143), (299, 7001)])
+def test_norm_odd_widths_between_powers_of_two(rows, C, dtype, layer, kept):
+    norm_case((rows, C), dtype, layer, kept, seed=C)
+
+
+@DTYPES
 @KEPT
 @pytest.mark.parametrize("rows,C", [(20011, 33), (1, 257), (9000, 511), (1300, 1023), (700, 2047), (301, 3001), (611, 4097),
                                     (150, 8191), (12, 8193)])
