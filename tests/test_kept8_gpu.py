@@ -1,4 +1,8 @@
 """8-bit kept activations, norms and SwiGLU on a B200 against 64-bit definitions."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -344,6 +348,22 @@ def test_linear(rows, K, N, bias):
     R.check(grads[1], d64.t() @ k64, torch.bfloat16, product_terms(d64.t(), k64), "dw")
     if bias:
         R.check(grads[2], d64.sum(0), torch.bfloat16, 1024 * R.F32 * d64.abs().sum(0), "db")
+
+
+def test_linear_backward_as_the_first_work_of_its_thread():
+    # a process of its own: autograd's thread keeps the CUDA context that earlier backwards left it
+    code = """
+import torch
+from pan2_b200.ops.kept8 import kept8_linear
+x = torch.ones(64, 256, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+w = torch.ones(128, 256, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+dy = torch.ones(64, 128, device="cuda", dtype=torch.bfloat16)
+dx, dw = torch.autograd.grad(kept8_linear(x, w), (x, w), dy)
+assert torch.equal(dx, torch.full_like(dx, 128)) and torch.equal(dw, torch.full_like(dw, 64))
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
 
 
 def test_linear_fp32_parameters_and_leading_dims():
