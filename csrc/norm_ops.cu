@@ -1404,7 +1404,7 @@ template <typename T, bool LAYER>
 void fwd_staged_any(const FwdCall& f) {
   const int C = f.a.C;
   constexpr bool B16 = sizeof(T) == 2;
-  constexpr int R = B16 ? 2 : 1, CTAS = B16 && LAYER ? 2 : 3, DEPTH = CTAS == 2 ? 6 : 4;
+  constexpr int R = B16 ? 2 : 1, CTAS = B16 ? 2 : 3, DEPTH = CTAS == 2 ? 6 : 4;
 #define STAGED(G) return fwd_staged<T, G, 2, R, DEPTH, CTAS, LAYER>(f)
 #define THIRDS(G) if constexpr (B16) if (C <= G * 24) return fwd_staged<T, G, 3, 1, 8, 2, LAYER>(f)
   if (C <= 64) STAGED(4);
