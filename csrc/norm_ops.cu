@@ -507,7 +507,8 @@ __global__ void __launch_bounds__(threads_of(G), CTAS)
 // issue: single elements are read, converted and masked (48 instructions an element in the forward of width 631), so
 // bf16 groups are sized for few idle lanes: 100 M elements, layer norm, kept forward / kept backward, two fragments of
 // twice the threads and then three a thread: width 333 269 / 250 and 210 / 182 us, 631 268 / 272 and 215 / 192, 77 291 / 249
-// and 213 / 191.
+// and 213 / 191.  Packed fp32 pairs cost more in moves than they save here (631: 226 / 217), and so does a branch for
+// whole fragments (230 / 225).
 constexpr int group_ctas(int G) { return G > kThreads ? 1 : 2; }
 constexpr int kGroupDepth = 3;
 
