@@ -1400,17 +1400,18 @@ bool fwd_flat(const FwdCall& f) {
   return true;
 }
 
-// A group holds 16 G columns; in bf16 rows of up to three quarters of that take groups of half the threads with three fragments
-// a thread (THIRDS), which leaves fewer idle.  100 M elements, layer norm, kept forward / kept backward, 16 G and then 24 G / 2:
-// width 384 124 / 129 and 89 / 110 us, 768 125 / 136 and 92 / 112, 1536 130 / 141 and 101 / 121, 6144 130 / 156 and 101 / 134.
-// In fp32 16 G reaches the same rate at 768 columns as at 1024.
+// A group holds 16 G columns; rows of up to three quarters of that take groups of half the threads with three fragments a
+// thread (THIRDS), which leaves fewer idle.  100 M bf16 elements, layer norm, kept forward / kept backward, 16 G and then
+// 24 G / 2: width 384 124 / 129 and 89 / 110 us, 768 125 / 136 and 92 / 112, 1536 130 / 141 and 101 / 121, 6144 130 / 156 and 101 / 134.
+// 50 M fp32, kept forward: width 264 101 and 82 us, 1280 85 and 74, 5120 105 and 76; the fp32 backward, whose rings of three
+// fragments hold two batches only, keeps 16 G (1280 104 us against 117).
 template <typename T, bool LAYER>
 void fwd_staged_any(const FwdCall& f) {
   const int C = f.a.C;
   constexpr bool B16 = sizeof(T) == 2;
   constexpr int R = B16 ? 2 : 1, CTAS = B16 ? 2 : 3, DEPTH = CTAS == 2 ? 6 : 4;
 #define STAGED(G) return fwd_staged<T, G, 2, R, DEPTH, CTAS, LAYER>(f)
-#define THIRDS(G) if constexpr (B16) if (C <= G * 24) return fwd_staged<T, G, 3, 1, 8, 2, LAYER>(f)
+#define THIRDS(G) if (C <= G * 24) return fwd_staged<T, G, 3, 1, B16 ? 8 : 4, 2, LAYER>(f)
   if (C <= 64) STAGED(4);
   if (C <= 128) STAGED(8);
   if (C <= 256) STAGED(16);
@@ -1578,7 +1579,7 @@ void bwd_wide(const BwdCall& b) {
   b.finish(parts);
 }
 
-// THIRDS as in the forward
+// THIRDS as in the forward, bf16 only
 template <typename T, bool LAYER, bool KEPT>
 void bwd_staged_any(const BwdCall& b) {
   const int C = b.a.C;
