@@ -236,8 +236,9 @@ GemmArgs base_args(const torch::Tensor& A, bool a_kmajor, torch::Tensor& D) {
   return a;
 }
 
+// `held` keeps what the launch reads besides the arguments.
 void set_group(GemmArgs& a, int g, const torch::Tensor& B, bool b_kmajor, int row_begin, int row_end,
-               const c10::optional<torch::Tensor>& bias) {
+               const c10::optional<torch::Tensor>& bias, std::vector<torch::Tensor>& held) {
   TORCH_CHECK(B.is_cuda() && B.scalar_type() == torch::kBFloat16 && B.dim() == 2 && B.stride(1) == 1,
               "B must be a row-major bf16 CUDA matrix");
   GemmGroup& gr = a.groups[g];
@@ -249,8 +250,10 @@ void set_group(GemmArgs& a, int g, const torch::Tensor& B, bool b_kmajor, int ro
   gr.row_end = row_end;
   gr.bias = nullptr;
   if (bias.has_value()) {
-    const auto& b = bias.value();
+    torch::Tensor b = bias.value();
     TORCH_CHECK(b.scalar_type() == torch::kBFloat16 && b.is_contiguous() && b.numel() >= gr.n, "bias must be bf16 [N]");
+    // the epilogue reads the bias 16 bytes at a time; a slice of a flat buffer may start between
+    if (reinterpret_cast<uintptr_t>(b.data_ptr()) % 16 != 0) held.push_back(b = b.clone());
     gr.bias = b.data_ptr();
   }
 }
@@ -263,7 +266,8 @@ void gemm(torch::Tensor A, torch::Tensor B, torch::Tensor D, bool a_kmajor, bool
   GemmArgs a = base_args(A, a_kmajor, D);
   a.b_mn = b_kmajor ? 0 : 1;
   a.n_groups = 1;
-  set_group(a, 0, B, b_kmajor, 0, a.M, bias);
+  std::vector<torch::Tensor> held;
+  set_group(a, 0, B, b_kmajor, 0, a.M, bias, held);
   TORCH_CHECK(a.groups[0].k == a.K, "K mismatch");
   TORCH_CHECK(D.size(0) >= a.M && D.size(1) >= a.groups[0].n, "D too small");
   if (gelu_pre.has_value()) {
@@ -338,12 +342,13 @@ void gemm_grouped_nt(torch::Tensor A, std::vector<torch::Tensor> Bs, torch::Tens
   a.b_mn = 0;
   int G = 0;
   int prev_end = -1;
+  std::vector<torch::Tensor> held;
   for (size_t g = 0; g + 1 < bounds.size(); ++g) {
     if (bounds[g + 1] <= bounds[g]) continue;
     TORCH_CHECK(G < kGemmMaxGroups, "at most 4 groups");
     TORCH_CHECK(prev_end < 0 || prev_end == bounds[g], "row groups must be contiguous");
     TORCH_CHECK(bounds[g + 1] <= a.M, "row bounds beyond A");
-    set_group(a, G, Bs[g], true, bounds[g], bounds[g + 1], g < biases.size() ? biases[g] : c10::nullopt);
+    set_group(a, G, Bs[g], true, bounds[g], bounds[g + 1], g < biases.size() ? biases[g] : c10::nullopt, held);
     TORCH_CHECK(D.size(1) >= a.groups[G].n, "D too narrow");
     prev_end = bounds[g + 1];
     ++G;
@@ -365,7 +370,8 @@ void gemm_dgelu(torch::Tensor dY, torch::Tensor Wd, torch::Tensor pre, torch::Te
   GemmArgs a = base_args(dY, true, dpre);
   a.b_mn = 1;
   a.n_groups = 1;
-  set_group(a, 0, Wd, false, 0, a.M, c10::nullopt);
+  std::vector<torch::Tensor> held;
+  set_group(a, 0, Wd, false, 0, a.M, c10::nullopt, held);
   TORCH_CHECK(a.groups[0].k == a.K, "K mismatch");
   TORCH_CHECK(pre.scalar_type() == torch::kBFloat16 && pre.stride(1) == 1 && post.stride(1) == 1, "bad pre/post");
   a.epi = 2;
