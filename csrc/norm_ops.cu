@@ -71,7 +71,7 @@ __device__ __forceinline__ void store_out(void* out, int c, float v) {
 }
 
 // ---------------------------------------------------------------- reductions
-// Sums of N values over each group of G threads; every thread of the group gets them.  `ws` holds
+// Sums of N values over each group of G threads; every thread of the group gets them.  `ws`, 16-byte aligned, holds
 // N floats a warp; calls that may overlap use different ones.  Inside a warp two values share each
 // exchange while there are two: a lane keeps one of a pair and hands over the other, so N values cost
 // N - 1 + log2(G) - log2(N) exchanges in place of N log2(G).
@@ -1059,7 +1059,7 @@ __global__ void __launch_bounds__(threads_of(G), single_ctas(G))
                            const float* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, void* dw,
                            void* db) {
   constexpr int NT = threads_of(G), GROUPS = NT / G;
-  __shared__ float ws[2][NT / 32 * 2 * R];
+  __shared__ __align__(16) float ws[2][NT / 32 * 2 * R];
   const int t = threadIdx.x % G, group = threadIdx.x / G, lane = threadIdx.x & 31;
   float w[E], aw[E], ab[E];
 #pragma unroll
@@ -1156,7 +1156,7 @@ __global__ void __launch_bounds__(32 * kFinalChains) norm_bwd_final_kernel(const
 
 // ---------------------------------------------------------------- rows too wide for registers
 __device__ __forceinline__ float cta_sum(float v) {
-  __shared__ float ws[kThreads / 32];
+  __shared__ __align__(16) float ws[kThreads / 32];
   __syncthreads();
   float s[1] = {v};
   group_sum<kThreads, 1>(s, ws);

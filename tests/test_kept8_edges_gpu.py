@@ -5,6 +5,7 @@ import torch
 
 import kept8_ref as R
 from pan2_b200.ops.kept8 import kept8_linear
+from pan2_b200.ops.norm import layer_norm, rms_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +47,49 @@ def test_linear_with_a_bias_at_an_odd_address(N, by):
     two, odd_two = torch.stack([b, b + 1]), odd_copy(torch.stack([b, b + 1]), by)
     ww = torch.stack([w, w])
     assert torch.equal(grouped_linear(x, ww, odd_two, [0, 100, 300]), grouped_linear(x, ww, two, [0, 100, 300]))
+
+
+# Views that are neither aligned nor contiguous: one element at a time, by groups of a warp (to 256 columns), of 256
+# threads (to 2048) and of 512 or 1024 (to 8192), then by sweeps.
+SINGLE = [(9, 200), (37, 257), (21, 1001), (300, 2048), (13, 2049), (8, 8191), (5, 9001), (3, 16400)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("layer", [True, False], ids=["layer", "rms"])
+@pytest.mark.parametrize("kept", [False, True], ids=["exact", "kept8"])
+@pytest.mark.parametrize("rows,C", SINGLE)
+def test_norm_of_views_of_every_width(rows, C, dtype, layer, kept):
+    view = lambda t: t[:, 1:1 + C]  # noqa: E731
+    base = R.activations(rows, C + 5, seed=C, dtype=dtype, device="cuda")
+    x = view(base).detach().requires_grad_(True)
+    gen = torch.Generator().manual_seed(C)
+    w = (1 + 0.3 * torch.randn(C, generator=gen)).to(dtype).cuda().requires_grad_(True)
+    b = (0.3 * torch.randn(C, generator=gen)).to(dtype).cuda().requires_grad_(True)
+    dy = view(torch.randn(rows, C + 5, generator=gen).to(dtype).cuda())
+    y = layer_norm(x, w, b, 1e-6, kept8=kept) if layer else rms_norm(x, w, 1e-6, kept8=kept)
+    wrt = (x, w, b) if layer else (x, w)
+    got = dict(zip(("dx", "dw", "db"), torch.autograd.grad(y, wrt, dy)), y=y)
+    ref = R.norm(x, w, b if layer else None, dy, 1e-6, layer, kept)
+    for name, t in got.items():
+        if name in ("y", "dx"):  # fp32 sums of at most 96 sequential terms and their tree, by the row's largest value
+            terms = 128 * R.F32 * ref[name].abs().amax(-1, keepdim=True)
+        else:  # at most 1024 sequential additions of terms that are off by some roundings
+            terms = 1024 * R.F32 * ref[name + "_abs"]
+        R.check(t, ref[name], dtype, terms, name)
+
+
+@pytest.mark.parametrize("by", [1, 2, 3])
+@pytest.mark.parametrize("C", [264, 1024, 4096])
+def test_norm_at_odd_addresses(C, by):
+    x, w, b, dy = bf16(40, C, seed=C), bf16(C, seed=1), bf16(C, seed=2), bf16(40, C, seed=3)
+    for kept in (False, True):
+        ref = R.norm(x, w, b, dy, 1e-6, True, kept)
+        for odd in ("x", "w", "dy", "all"):
+            args = {n: odd_copy(t, by) if odd in (n, "all") else t for n, t in (("x", x), ("w", w), ("b", b), ("dy", dy))}
+            xs, ws, bs = (args[n].detach().requires_grad_(True) for n in ("x", "w", "b"))
+            y = layer_norm(xs, ws, bs, kept8=kept)
+            got = dict(zip(("dx", "dw", "db"), torch.autograd.grad(y, (xs, ws, bs), args["dy"])), y=y)
+            for name, t in got.items():
+                terms = (128 * R.F32 * ref[name].abs().amax(-1, keepdim=True) if name in ("y", "dx")
+                         else 1024 * R.F32 * ref[name + "_abs"])
+                R.check(t, ref[name], torch.bfloat16, terms, f"{name}, {odd} odd")
