@@ -419,6 +419,7 @@ __global__ void __launch_bounds__(kThreads) swiglu_fwd_flat_kernel(const T* gate
     uint32_t r;
     int c;
     flat_frag<V>(t, f, act ? u : 0, r, c);
+    if (!act) c = f.cols;  // reads nothing: the first fragment's thread writes h over its values meanwhile
     float g[V], v[V];
     if constexpr (sizeof(T) == 2) {
       Piece<T, 8> pg, pv;
