@@ -106,7 +106,9 @@ class BlockCheckpoint(torch.autograd.Function):
         ctx.engine, ctx.idx = engine, idx
         stash = engine.stash_checkpoint(idx, x, ln_stats)
         ctx.kept = None
-        if stash is None and engine.checkpoint_bits == 8:
+        # a kept attention output is that of the exact x: joined to q, k, v recomputed from 8 bits, it would make the
+        # gradient of no forward (probabilities that do not sum to 1)
+        if stash is None and engine.checkpoint_bits == 8 and not engine.keep_attention:
             kept = keep8(x)
             ctx.save_for_backward(kept.codes, kept.scales, ln_stats, vec)
             ctx.kept, ctx.stash = (kept.shape, kept.dtype), None
@@ -471,7 +473,8 @@ class TrainEngine:
 
         ``bits=8`` keeps activations in 8 bits (:mod:`pan2_b200.ops.kept8`): block checkpoints that take
         memory of their own (those parked in idle gradient buffers stay as they are: they are free and
-        exact), and the caption path's norm, projection and SwiGLU inputs.  The forward is exact up to the
+        exact; so do all with ``keep_attention``, whose kept outputs belong to the exact inputs), and the
+        caption path's norm, projection and SwiGLU inputs.  The forward is exact up to the
         fused norms' single rounding; gradients carry the store's error (about 1 % of a block's values)."""
         if bits not in (8, 16):
             raise ValueError(f"activations are kept in 16 or 8 bits, not {bits}")

@@ -92,3 +92,21 @@ def test_options():
         cfg.check()
     with pytest.raises(ValueError, match="16 or 8"):
         _engine(4)
+
+
+def test_kept_attention_leaves_the_checkpoints_exact(monkeypatch):
+    """The kept attention output belongs to the exact input: a recompute from 8 bits would join it to other q, k, v."""
+    from pan2_b200.training import engine as E
+    calls = []
+    monkeypatch.setattr(E, "keep8", lambda x, _keep=E.keep8: calls.append(x.shape) or _keep(x))
+    eng = _engine(16)
+    batch, _ = tiny_batch(eng.model, seed=7)
+    _, exact = _grads(eng, batch)
+    eng = _engine(8)
+    eng.set_activation_checkpointing(True, keep_attention=True, bits=8)
+    _, kept = _grads(eng, batch)
+    assert not calls and eng.model.kept8
+    for name, g in exact.items():
+        if name.startswith("blocks.") and float(g.norm()) > 0:
+            # the joint blocks see the fused norms' rounding in the captions, nothing else
+            assert float((kept[name] - g).norm() / g.norm()) < 1e-3, name

@@ -63,3 +63,27 @@ def test_caption_encoder_holds_less_memory():
     assert float((out[True] - out[False]).norm() / out[False].norm()) < 2e-2  # norms round once instead of twice
     assert float(torch.nn.functional.cosine_similarity(grads[True], grads[False], dim=0)) > 0.99
     assert held[True] < 0.5 * held[False], held
+
+
+def test_kept_attention_with_8_bits_follows_the_exact_step(monkeypatch):
+    """Attention outputs kept by the forward are those of the exact input, so the blocks' checkpoints stay exact."""
+    from pan2_b200.data.synthetic import batch_to_device
+    from pan2_b200.training import engine as E
+    calls, grads = [], {}
+    monkeypatch.setattr(E, "keep8", lambda x, _keep=E.keep8: calls.append(x.shape) or _keep(x))
+    for bits in (16, 8):
+        eng = E.TrainEngine(ARCH, torch.device("cuda"), seed=5, optim=E.OptimConfig(lr=1e-3), offload="off")
+        eng.set_activation_checkpointing(True, keep_attention=True, bits=bits)
+        eng.stash_in_grads = False
+        batch, _ = tiny_batch(eng.model)
+        b = batch_to_device(batch, "cuda")
+        for k in ("hidden_states", "text_states", "target"):
+            b[k] = b[k].to(torch.bfloat16)
+        eng.forward_backward(b)
+        grads[bits] = {s.name: u.slot_full(u.full_grad, s).float().clone() for u in eng.sharded.units for s in u.slots}
+        del eng
+    assert not calls
+    for name, g in grads[16].items():
+        if float(g.norm()) > 0:
+            cos = float(torch.nn.functional.cosine_similarity(g.flatten(), grads[8][name].flatten(), dim=0))
+            assert cos > 0.99, (name, cos)
