@@ -37,9 +37,10 @@ void check_launch(const char* err, const char* what) {
   TORCH_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e));
 }
 
-}  // namespace
-
-namespace {
+// The kernels' gradients carry no graph: a backward that is itself to be differentiated would drop terms in silence.
+void refuse_create_graph(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, " has no second derivative: run its backward without create_graph");
+}
 
 // A tensor as rows of its last dimension; a copy is made only where the leading dimensions do not
 // collapse to two strided levels or the last dimension is not adjacent in memory.
@@ -262,6 +263,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     const variable_list saved = ctx->get_saved_variables();
     const int64_t flags = ctx->saved_data["flags"].toInt();
     const bool layer = flags & 4, w_fp32 = flags & 8;
+    refuse_create_graph(layer ? "layer_norm" : "rms_norm");
     const bool need_dx = ctx->needs_input_grad(0), need_dw = (flags & 1) && ctx->needs_input_grad(1),
                need_db = (flags & 2) && ctx->needs_input_grad(flags & 1 ? 2 : 1);  // missing vectors have no edge
     const at::cuda::CUDAGuard guard(dy_.device());
@@ -395,6 +397,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_create_graph("kept8_linear");
     const torch::Tensor& gy = grads[0];
     const at::cuda::CUDAGuard guard(gy.device());
     const variable_list saved = ctx->get_saved_variables();
@@ -426,6 +429,7 @@ struct SwiGLUNode : torch::autograd::Function<SwiGLUNode> {
     return out[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_create_graph("kept8_swiglu");
     const variable_list k = ctx->get_saved_variables();
     auto out = swiglu8_bwd(grads[0], k[0], k[1], k[2], k[3], false);
     return {out[0], out[1], torch::Tensor()};

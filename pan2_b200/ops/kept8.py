@@ -19,7 +19,8 @@ Format: every row is cut into blocks of 32 consecutive channels; a block has one
 infinity or a NaN read back as NaN, so a non-finite activation still reaches the gradients.
 
 Gradients are those of the formulas evaluated at the kept values; the store itself is treated as the
-identity (no gradient flows through the rounding).  CUDA tensors run the sm_100a kernels of
+identity (no gradient flows through the rounding).  There are no second derivatives: a backward with
+``create_graph=True`` raises, since codes and statistics carry no graph.  CUDA tensors run the sm_100a kernels of
 ``csrc/kept8_ops.cu`` and ``csrc/gemm_sm100.cu``; CPU tensors run plain PyTorch with the same math.
 """
 from __future__ import annotations
@@ -73,6 +74,12 @@ def _check_match(a: torch.Tensor, b: torch.Tensor, names: str) -> None:
     if a.shape != b.shape or a.dtype != b.dtype or a.device != b.device:
         raise ValueError(f"{names} differ: {tuple(a.shape)} {a.dtype} {a.device} and "
                          f"{tuple(b.shape)} {b.dtype} {b.device}")
+
+
+def refuse_create_graph(name: str) -> None:
+    """Raise in a backward that is itself to be differentiated (what it reads carries no graph)."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{name} has no second derivative: run its backward without create_graph")
 
 
 def wide_dtype(dtype: torch.dtype) -> torch.dtype:
@@ -228,6 +235,7 @@ class _Kept8LinearCPU(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gy):
+        refuse_create_graph("kept8_linear")
         codes, scales, w = ctx.saved_tensors
         g2 = gy.reshape(-1, gy.shape[-1])
         gx = _input_grad(g2, w).reshape(ctx.shape) if ctx.needs_input_grad[0] else None
@@ -282,6 +290,7 @@ class _Kept8SwiGLUCPU(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dh):
+        refuse_create_graph("kept8_swiglu")
         return tuple(_swiglu_backward(dh, ctx.saved_tensors, False))
 
 
@@ -308,6 +317,7 @@ class _Kept8SwiGLUFFN(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gy):
+        refuse_create_graph("kept8_swiglu_ffn")
         codes, scales, *kept, w1, w3, w2 = ctx.saved_tensors
         need_x, need_1, need_3, need_2 = ctx.needs_input_grad
         g2 = gy.reshape(-1, gy.shape[-1])

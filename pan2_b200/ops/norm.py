@@ -6,7 +6,8 @@ rounds ``n`` before the weight multiplies it.
 
 The backward returns ``dx`` and the fully reduced ``dw`` / ``db`` (fp32 sums in a fixed order: the same
 bits every time).  With ``kept8=True`` the input is kept in 8 bits (:mod:`pan2_b200.ops.kept8`) and the
-backward reads ``n`` from those, with the exact input's ``mean`` and ``rstd``.
+backward reads ``n`` from those, with the exact input's ``mean`` and ``rstd``.  There are no second
+derivatives: a backward with ``create_graph=True`` raises.
 
 CUDA tensors (bf16 or fp32; any width, any leading dims, strided rows without a copy) run the
 sm_100a kernels of ``csrc/norm_ops.cu``; CPU tensors run plain PyTorch with the same math.
@@ -18,7 +19,7 @@ from typing import Optional
 import torch
 
 from ._ext import ext
-from .kept8 import _keep_cpu, _values_cpu, check_activation, wide_dtype
+from .kept8 import _keep_cpu, _values_cpu, check_activation, refuse_create_graph, wide_dtype
 
 
 class _NormCPU(torch.autograd.Function):
@@ -33,6 +34,7 @@ class _NormCPU(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        refuse_create_graph("layer_norm" if ctx.layer else "rms_norm")
         x, codes, scales, stats, w = ctx.saved_tensors
         grads = _backward_cpu(dy, x, codes, scales, stats, w, ctx.layer, ctx.w_dtype)
         return *(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None

@@ -170,3 +170,32 @@ def test_refusals():
     with pytest.raises(ValueError, match="negative"):
         rms_norm(x, eps=float("nan"))
     assert isinstance(keep8(x), Kept8)
+
+
+def kept_calls(dtype, device, grad=True):
+    """Every operator with a backward, on small inputs: ``name -> (call, inputs)``."""
+    t = lambda *s: R.activations(*s, seed=len(s), dtype=dtype, device=device).requires_grad_(grad)  # noqa: E731
+    return {
+        "layer_norm": (layer_norm, (t(4, 64), t(64), t(64))),
+        "layer_norm kept8": (lambda *a: layer_norm(*a, kept8=True), (t(4, 64), t(64), t(64))),
+        "rms_norm": (rms_norm, (t(4, 64), t(64))),
+        "rms_norm kept8": (lambda *a: rms_norm(*a, kept8=True), (t(4, 64), t(64))),
+        "kept8_linear": (kept8_linear, (t(4, 64), t(8, 64))),
+        "kept8_swiglu": (kept8_swiglu, (t(4, 64), t(4, 64))),
+        "kept8_swiglu_ffn": (kept8_swiglu_ffn, (t(4, 64), t(96, 64), t(96, 64), t(64, 96))),
+    }
+
+
+def refuses_second_derivatives(dtype, device):
+    for name, (call, inputs) in kept_calls(dtype, device).items():
+        y = call(*inputs)
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            torch.autograd.grad(y.float().sum(), inputs, create_graph=True)
+        grads = torch.autograd.grad(call(*inputs).float().sum(), inputs)  # as before without
+        assert all(g.shape == i.shape and not g.requires_grad for g, i in zip(grads, inputs)), name
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_second_derivatives_are_refused(dtype):
+    """The backward reads statistics and codes that carry no graph, so what it returns must not be differentiated."""
+    refuses_second_derivatives(dtype, "cpu")

@@ -93,3 +93,9 @@ def test_norm_at_odd_addresses(C, by):
                 terms = (128 * R.F32 * ref[name].abs().amax(-1, keepdim=True) if name in ("y", "dx")
                          else 1024 * R.F32 * ref[name + "_abs"])
                 R.check(t, ref[name], torch.bfloat16, terms, f"{name}, {odd} odd")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_second_derivatives_are_refused(dtype):
+    from test_kept8_cpu import refuses_second_derivatives
+    refuses_second_derivatives(dtype, "cuda")
