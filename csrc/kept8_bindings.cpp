@@ -115,7 +115,7 @@ Kept8Buf kept_of(const torch::Tensor& codes, const torch::Tensor& scales, int64_
 }
 
 void check_same(const RowsOf& a, const RowsOf& b, const char* what) {
-  TORCH_CHECK_VALUE(a.rows == b.rows && a.C == b.C && a.fp32 == b.fp32 && a.t.device() == b.t.device(), what,
+  TORCH_CHECK_VALUE(a.t.sizes() == b.t.sizes() && a.fp32 == b.fp32 && a.t.device() == b.t.device(), what,
                     " differ: ", shape_text(a.t), " ", type_text(a.t), " ", device_text(a.t), " and ", shape_text(b.t), " ",
                     type_text(b.t), " ", device_text(b.t));
 }

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import kept8_ref as R
-from pan2_b200.ops.kept8 import kept8_linear
+from pan2_b200.ops.kept8 import kept8_linear, kept8_swiglu
 from pan2_b200.ops.norm import layer_norm, rms_norm
 
 pytestmark = pytest.mark.gpu
@@ -99,3 +99,13 @@ def test_norm_at_odd_addresses(C, by):
 def test_second_derivatives_are_refused(dtype):
     from test_kept8_cpu import refuses_second_derivatives
     refuses_second_derivatives(dtype, "cuda")
+
+
+def test_swiglu_refuses_shapes_that_only_have_as_many_rows():
+    gate = torch.randn(4, 64, device="cuda", requires_grad=True)
+    for shape in ((2, 2, 64), (1, 4, 64)):
+        for pair in ((gate, torch.randn(shape, device="cuda")), (torch.randn(shape, device="cuda"), gate)):
+            with pytest.raises(ValueError, match="differ"):
+                kept8_swiglu(*pair)
+            with pytest.raises(ValueError, match="differ"):  # as the CPU path does
+                kept8_swiglu(*(t.cpu() for t in pair))
