@@ -472,6 +472,14 @@ torch::Tensor swiglu8(torch::Tensor gate, torch::Tensor value) {
   return SwiGLUNode::apply(gate, value, at::GradMode::is_enabled() && (gate.requires_grad() || value.requires_grad()));
 }
 
+// A matrix or a weight as an operand of the products, for nodes that run several (Python).
+torch::Tensor gemm_operand(torch::Tensor t, bool weight) {
+  const at::cuda::CUDAGuard guard(t.device());
+  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && (weight || t.scalar_type() == torch::kBFloat16),
+              "gemm_operand: a bf16 CUDA matrix, or a weight");
+  return weight ? weight_operand(t) : operand(t);
+}
+
 // dW [N, K] of one projection from its kept input, for nodes that hold several (Python).
 torch::Tensor linear8_weight_grad(torch::Tensor g2, torch::Tensor codes, torch::Tensor scales, int64_t K, bool fp32) {
   const at::cuda::CUDAGuard guard(g2.device());
@@ -507,6 +515,7 @@ void bind_kept8(pybind11::module_& m) {
   m.def("row_sum", &row_sum, kNoGil);
   m.def("norm", &norm, kNoGil);
   m.def("linear8", &linear8, kNoGil);
+  m.def("gemm_operand", &gemm_operand, kNoGil);
   m.def("linear8_weight_grad", &linear8_weight_grad, kNoGil);
 }
 

@@ -30,7 +30,7 @@ from typing import Optional, Tuple
 import torch
 
 from ._ext import ext
-from .gemm import _pad_k, mm_nn, mm_nt
+from .gemm import mm_nn, mm_nt
 
 BLOCK = 32
 
@@ -145,28 +145,6 @@ def restore8(kept: Kept8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
 # linear
 # --------------------------------------------------------------------------------------------
 
-def _pad8(n: int) -> int:
-    return (n + 7) // 8 * 8
-
-
-def _weight_operand(w: torch.Tensor) -> torch.Tensor:
-    """``w`` as the GEMMs read it: bf16, rows and columns zero-padded to multiples of 8."""
-    N, K = w.shape
-    w = w.to(torch.bfloat16)
-    if N % 8 == 0 and K % 8 == 0:
-        return w.contiguous()
-    out = w.new_zeros(_pad8(N), _pad8(K))
-    out[:N, :K] = w
-    return out
-
-
-def _bias_operand(b: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    if b is None:
-        return None
-    b = b.to(torch.bfloat16)
-    return torch.nn.functional.pad(b, (0, _pad8(b.shape[0]) - b.shape[0])).contiguous()
-
-
 def weight_grad8(g: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, K: int, dtype) -> torch.Tensor:
     """``g^T x`` in ``dtype``, ``x [rows, K]`` the kept matrix and ``g [rows, N]``: the weight gradient of a
     projection that read ``x``."""
@@ -183,28 +161,31 @@ def row_sum(g: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return g.to(wide_dtype(g.dtype)).sum(0).to(dtype)
 
 
-def _project(x2: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor]) -> torch.Tensor:
-    """``x2 [rows, K] @ w^T + b`` (no autograd)."""
-    N, K = w.shape
+def _project(x2: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+    """``x2 [rows, K] @ w^T`` (no autograd)."""
     if not x2.is_cuda:
-        wide = wide_dtype(x2.dtype)
-        y = x2.to(wide) @ w.to(wide).t()
-        return (y if b is None else y + b.to(wide)).to(x2.dtype)
+        return _project_cpu(x2, w, None)
     if x2.shape[0] == 0:
-        return x2.new_empty(0, N)
-    return mm_nt(_pad_k(x2, _pad8(K)), _weight_operand(w), bias=_bias_operand(b))[:, :N]
+        return x2.new_empty(0, w.shape[0])
+    return mm_nt(ext().gemm_operand(x2, False), ext().gemm_operand(w, True))[:, :w.shape[0]]
+
+
+def _project_cpu(x2: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor]) -> torch.Tensor:
+    wide = wide_dtype(x2.dtype)
+    y = x2.to(wide) @ w.to(wide).t()
+    return (y if b is None else y + b.to(wide)).to(x2.dtype)
 
 
 def _input_grad(g2: torch.Tensor, w: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``g2 [rows, N] @ w`` (added to ``out`` when given)."""
-    N, K = w.shape
+    K = w.shape[1]
     if not g2.is_cuda:
         wide = wide_dtype(g2.dtype)
         y = (g2.to(wide) @ w.to(wide)).to(g2.dtype)
         return y if out is None else out + y
     if g2.shape[0] == 0:
         return g2.new_empty(0, K)
-    gp, wp = _pad_k(g2, _pad8(N)), _weight_operand(w)
+    gp, wp = ext().gemm_operand(g2, False), ext().gemm_operand(w, True)
     if out is None:
         return mm_nn(gp, wp)[:, :K]
     if K % 8 == 0:
@@ -227,7 +208,7 @@ class _Kept8LinearCPU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b):
         x2 = x.reshape(-1, x.shape[-1])
-        y = _project(x2, w, b)
+        y = _project_cpu(x2, w, b)
         codes, scales = _keep_cpu(x2) if ctx.needs_input_grad[1] else (None, None)
         ctx.save_for_backward(codes, scales, w)
         ctx.shape, ctx.b_dtype = x.shape, None if b is None else b.dtype
@@ -310,10 +291,10 @@ class _Kept8SwiGLUFFN(torch.autograd.Function):
     def forward(ctx, x, w1, w3, w2):
         K = x.shape[-1]
         x2 = x.reshape(-1, K)
-        h, *kept = _swiglu_forward(_project(x2, w1, None), _project(x2, w3, None))
+        h, *kept = _swiglu_forward(_project(x2, w1), _project(x2, w3))
         ctx.save_for_backward(*keep_codes(x2), *kept, w1, w3, w2)
         ctx.shape = x.shape
-        return _project(h, w2, None).reshape(*x.shape[:-1], w2.shape[0])
+        return _project(h, w2).reshape(*x.shape[:-1], w2.shape[0])
 
     @staticmethod
     def backward(ctx, gy):
@@ -354,6 +335,6 @@ def kept8_swiglu_ffn(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: to
         x = x.to(torch.bfloat16)
     if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, w1, w3, w2))):  # nothing to keep
         x2 = x.reshape(-1, x.shape[-1])
-        h = kept8_swiglu(_project(x2, w1, None), _project(x2, w3, None))
-        return _project(h, w2, None).reshape(*x.shape[:-1], w2.shape[0])
+        h = kept8_swiglu(_project(x2, w1), _project(x2, w3))
+        return _project(h, w2).reshape(*x.shape[:-1], w2.shape[0])
     return _Kept8SwiGLUFFN.apply(x, w1, w3, w2)

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import kept8_ref as R
-from pan2_b200.ops.kept8 import kept8_linear, kept8_swiglu
+from pan2_b200.ops.kept8 import kept8_linear, kept8_swiglu, kept8_swiglu_ffn
 from pan2_b200.ops.norm import layer_norm, rms_norm
 
 pytestmark = pytest.mark.gpu
@@ -109,3 +109,25 @@ def test_swiglu_refuses_shapes_that_only_have_as_many_rows():
                 kept8_swiglu(*pair)
             with pytest.raises(ValueError, match="differ"):  # as the CPU path does
                 kept8_swiglu(*(t.cpu() for t in pair))
+
+
+def test_swiglu_ffn_at_odd_addresses():
+    x, dy = bf16(120, 64, seed=1), bf16(120, 40, seed=5)
+    w1, w3, w2 = bf16(96, 64, seed=2, scale=0.125), bf16(96, 64, seed=3, scale=0.125), bf16(40, 96, seed=4, scale=0.125)
+
+    def run(*args):
+        *args, g = args
+        args = [a.detach().requires_grad_(True) for a in args]
+        y = kept8_swiglu_ffn(*args)
+        return (y, *torch.autograd.grad(y, args, g))
+    want = run(x, w1, w3, w2, dy)
+    names = ("x", "w1", "w3", "w2", "dy")
+    for which in names + ("all",):
+        args = [odd_copy(t, 3) if which in (n, "all") else t for n, t in zip(names, (x, w1, w3, w2, dy))]
+        for a, b, name in zip(want, run(*args), ("y", "dx", "dw1", "dw3", "dw2")):
+            assert torch.equal(a, b), (which, name)
+    wide = bf16(120, 130, seed=1)  # a column slice with rows at odd addresses
+    for a, b in zip(run(wide[:, 1:65].contiguous(), w1, w3, w2, dy), run(wide[:, 1:65], w1, w3, w2, dy)):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        assert torch.equal(kept8_swiglu_ffn(odd_copy(x), w1, w3, w2), want[0])
