@@ -176,21 +176,20 @@ def _project_cpu(x2: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor]) -
     return (y if b is None else y + b.to(wide)).to(x2.dtype)
 
 
-def _input_grad(g2: torch.Tensor, w: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``g2 [rows, N] @ w`` (added to ``out`` when given)."""
-    K = w.shape[1]
-    if not g2.is_cuda:
-        wide = wide_dtype(g2.dtype)
-        y = (g2.to(wide) @ w.to(wide)).to(g2.dtype)
-        return y if out is None else out + y
-    if g2.shape[0] == 0:
-        return g2.new_empty(0, K)
-    gp, wp = ext().gemm_operand(g2, False), ext().gemm_operand(w, True)
-    if out is None:
-        return mm_nn(gp, wp)[:, :K]
-    if K % 8 == 0:
-        return mm_nn(gp, wp, out=out, accumulate=True)
-    return out + mm_nn(gp, wp)[:, :K]
+def _input_grad(*pairs: Tuple[torch.Tensor, torch.Tensor]) -> torch.Tensor:
+    """Sum of ``g2 [rows, N] @ w [N, K]`` over the pairs.  On CUDA the sum so far is bf16 between the products (one
+    rounding more than an fp32 sum, at half its traffic); the next one is added to it in fp32."""
+    out = None
+    for g2, w in pairs:
+        if not g2.is_cuda:
+            wide = wide_dtype(g2.dtype)
+            y = (g2.to(wide) @ w.to(wide)).to(g2.dtype)
+            out = y if out is None else out + y
+        elif g2.shape[0] == 0:
+            out = g2.new_empty(0, w.shape[1])
+        else:
+            out = mm_nn(ext().gemm_operand(g2, False), ext().gemm_operand(w, True), out=out, accumulate=out is not None)
+    return out[:, :pairs[0][1].shape[1]]
 
 
 def _check_linear(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor]) -> None:
@@ -219,7 +218,7 @@ class _Kept8LinearCPU(torch.autograd.Function):
         refuse_create_graph("kept8_linear")
         codes, scales, w = ctx.saved_tensors
         g2 = gy.reshape(-1, gy.shape[-1])
-        gx = _input_grad(g2, w).reshape(ctx.shape) if ctx.needs_input_grad[0] else None
+        gx = _input_grad((g2, w)).reshape(ctx.shape) if ctx.needs_input_grad[0] else None
         gw = weight_grad8(g2, codes, scales, w.shape[1], w.dtype) if ctx.needs_input_grad[1] else None
         gb = row_sum(g2, ctx.b_dtype) if ctx.b_dtype is not None and ctx.needs_input_grad[2] else None
         return gx, gw, gb
@@ -302,12 +301,12 @@ class _Kept8SwiGLUFFN(torch.autograd.Function):
         codes, scales, *kept, w1, w3, w2 = ctx.saved_tensors
         need_x, need_1, need_3, need_2 = ctx.needs_input_grad
         g2 = gy.reshape(-1, gy.shape[-1])
-        dgate, dvalue, *h = _swiglu_backward(_input_grad(g2, w2).contiguous(), kept, need_2)
+        dgate, dvalue, *h = _swiglu_backward(_input_grad((g2, w2)).contiguous(), kept, need_2)
         gx = gw1 = gw3 = gw2 = None
         if need_2:
             gw2 = _dense_weight_grad(g2, h[0], w2.dtype)
         if need_x:
-            gx = _input_grad(dvalue, w3, out=_input_grad(dgate, w1)).reshape(ctx.shape)
+            gx = _input_grad((dgate, w1), (dvalue, w3)).reshape(ctx.shape)
         if need_1:
             gw1 = weight_grad8(dgate, codes, scales, w1.shape[1], w1.dtype)
         if need_3:

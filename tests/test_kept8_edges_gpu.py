@@ -111,6 +111,49 @@ def test_swiglu_refuses_shapes_that_only_have_as_many_rows():
                 kept8_swiglu(*(t.cpu() for t in pair))
 
 
+def product_terms(a, b):
+    """Bound on the fp32 accumulation error of ``a @ b``: the terms' absolute sum, 64 roundings."""
+    return 64 * R.F32 * (a.abs() @ b.abs())
+
+
+def d(t):
+    return t.detach().cpu().double()
+
+
+@pytest.mark.parametrize("w_dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("rows,K,H,N", [(260, 96, 328, 96), (77, 100, 171, 45), (300, 33, 1001, 64), (1, 64, 8, 200),
+                                        (0, 64, 96, 40)])
+def test_swiglu_ffn_against_64_bits(rows, K, H, N, w_dtype):
+    """Each step against 64 bits, given the inputs that the step before it makes: the same kernels on the same
+    operands as inside the FFN, so its bf16 intermediates are at hand."""
+    from pan2_b200.ops._ext import ext
+    x = bf16(rows, K, seed=1).requires_grad_(True)
+    # values of bf16 in either type: fp32 weights are read as bf16
+    w1, w3 = (bf16(H, K, seed=s, scale=K ** -0.5).to(w_dtype).requires_grad_(True) for s in (2, 3))
+    w2 = bf16(N, H, seed=4, scale=H ** -0.5).to(w_dtype).requires_grad_(True)
+    dy = bf16(rows, N, seed=5)
+    y = kept8_swiglu_ffn(x, w1, w3, w2)
+    dx, dw1, dw3, dw2 = torch.autograd.grad(y, (x, w1, w3, w2), dy)
+    assert [t.dtype for t in (y, dx, dw1, dw3, dw2)] == [torch.bfloat16] * 2 + [w_dtype] * 3
+    gate, value = kept8_linear(x, w1).detach(), kept8_linear(x, w3).detach()
+    h, *kept = ext().swiglu8_fwd(gate, value, True)
+    R.check(y, d(h) @ d(w2).t(), torch.bfloat16, product_terms(d(h), d(w2).t()), "y")
+    hh = h.clone().requires_grad_(True)
+    (dh,) = torch.autograd.grad(kept8_linear(hh, w2), hh, dy)
+    dgate, dvalue = ext().swiglu8_bwd(dh, *kept, False)
+    k64 = R.kept_values(x)
+    for got, by, name in ((dw1, dgate, "dw1"), (dw3, dvalue, "dw3")):
+        R.check(got, d(by).t() @ k64, w_dtype, product_terms(d(by).t(), k64), name)
+    one, two = d(dgate) @ d(w1), d(dvalue) @ d(w3)
+    # the first product is rounded to bf16 before the second is added to it
+    R.check(dx, one + two, torch.bfloat16,
+            2 * R.BF16 * one.abs() + product_terms(d(dgate), d(w1)) + product_terms(d(dvalue), d(w3)), "dx")
+    # the product of the kept values, rounded to bf16: a handful of fp32 roundings before that
+    h64 = R.swiglu(gate, value, dh)["kept_h"] if rows else torch.zeros(0, H, dtype=torch.double)
+    off = 2 * R.BF16 * h64.abs() + 32 * R.F32 * (R.kept_values(gate) * R.kept_values(value)).abs()
+    R.check(dw2, d(dy).t() @ h64, w_dtype, d(dy).abs().t() @ off + product_terms(d(dy).t(), h64), "dw2")
+
+
 def test_swiglu_ffn_at_odd_addresses():
     x, dy = bf16(120, 64, seed=1), bf16(120, 40, seed=5)
     w1, w3, w2 = bf16(96, 64, seed=2, scale=0.125), bf16(96, 64, seed=3, scale=0.125), bf16(40, 96, seed=4, scale=0.125)
