@@ -26,6 +26,7 @@
 #include "gemm_host.h"
 #include "launchers.h"
 #include "sm100.cuh"
+#include "smem_opt_in.h"
 
 namespace pan {
 namespace gemm {
@@ -644,13 +645,9 @@ const char* launch_gemm(const GemmArgs& a, cudaStream_t stream) {
   if (tiles == 0) return nullptr;
   p.probe = g_probe;
   if (cg == 1) {
-    static bool attr1 = false;
-    if (!attr1) {
-      if (cudaFuncSetAttribute(gemm_kernel<1, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               Cfg<1, 4>::SMEM_BYTES) != cudaSuccess)
-        return "gemm: cannot set the dynamic shared memory size";
-      attr1 = true;
-    }
+    static SmemOptIn opted;
+    if (!allow_smem(opted, gemm_kernel<1, 4>, Cfg<1, 4>::SMEM_BYTES))
+      return "gemm: cannot set the dynamic shared memory size";
     const int grid = tiles < num_sms() ? tiles : num_sms();
     gemm_kernel<1, 4><<<grid, kThreads, Cfg<1, 4>::SMEM_BYTES, stream>>>(p, maps);
   } else {
@@ -670,13 +667,9 @@ const char* launch_gemm(const GemmArgs& a, cudaStream_t stream) {
     switch (g_pair_stages) {
 #define PAN_PAIR_LAUNCH(S)                                                                                         \
   case S: {                                                                                                      \
-    static bool set = false;                                                                                     \
-    if (!set) {                                                                                                  \
-      if (cudaFuncSetAttribute(gemm_kernel<2, S>, cudaFuncAttributeMaxDynamicSharedMemorySize,                   \
-                               Cfg<2, S>::SMEM_BYTES) != cudaSuccess)                                            \
-        return "gemm: cannot set the dynamic shared memory size";                                                \
-      set = true;                                                                                                \
-    }                                                                                                            \
+    static SmemOptIn opted;                                                                                      \
+    if (!allow_smem(opted, gemm_kernel<2, S>, Cfg<2, S>::SMEM_BYTES))                                            \
+      return "gemm: cannot set the dynamic shared memory size";                                                  \
     cfg.dynamicSmemBytes = Cfg<2, S>::SMEM_BYTES;                                                                \
     e = cudaLaunchKernelEx(&cfg, gemm_kernel<2, S>, p, maps);                                                    \
     break;                                                                                                       \

@@ -20,6 +20,7 @@
 #include "flat.cuh"
 #include "kept8.cuh"
 #include "launchers.h"
+#include "smem_opt_in.h"
 
 namespace pan {
 namespace {
@@ -1305,8 +1306,8 @@ void fwd_staged(const FwdCall& f) {
   constexpr int NT = threads_of(G), GROUPS = NT / G, BYTES = DEPTH * Ring<T, NT, R * UPT>::STAGE;
   static_assert(BYTES * CTAS <= kRingBudget, "the rings of an SM's CTAs do not fit its shared memory");
   const auto kernel = norm_fwd_staged_kernel<T, G, UPT, R, DEPTH, CTAS, LAYER>;
-  static bool ready = false;
-  if (!ready) ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) == cudaSuccess;
+  static SmemOptIn opted;
+  allow_smem(opted, kernel, BYTES);
   kernel<<<grid_for(f.a.rows, GROUPS * R, CTAS), NT, BYTES, f.s>>>(view_of(f.x), (uint32_t)f.a.rows, f.a.C, f.vec(),
                                                                    f.a.eps, (T*)f.y, f.stats, kept_of(f.k));
 }
@@ -1324,8 +1325,8 @@ void fwd_group(const FwdCall& f) {
   constexpr int BYTES = kGroupDepth * B::ROOM;
   static_assert(BYTES * group_ctas(G) <= kRingBudget, "the batches of an SM's CTAs do not fit its shared memory");
   const auto kernel = norm_fwd_flat_kernel<T, G, UPT, R>;
-  static bool ready = false;
-  if (!ready) ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) == cudaSuccess;
+  static SmemOptIn opted;
+  allow_smem(opted, kernel, BYTES);
   kernel<<<grid_for(f.a.rows, B::ROWS, group_ctas(G)), B::NT, BYTES, f.s>>>((const T*)f.x.p, (uint32_t)f.a.rows, f.a.C,
                                                                            f.vec(), f.a.eps, f.a.layer, (T*)f.y,
                                                                            f.stats, kept_of(f.k));
@@ -1360,12 +1361,6 @@ FlatPlan flat_plan(int C, int esize, int tensors, bool kept, int vectors, int wa
 }
 int flat_bytes(const FlatPlan& p, int C, int vectors) { return (int)(p.vectors + ((size_t)vectors * C + 4) * 4 + p.rows * 16); }
 
-template <typename K>
-void allow_smem(K kernel, int bytes, int& allowed) {
-  if (bytes > allowed && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess)
-    allowed = bytes;
-}
-
 template <typename T>
 bool fwd_flat(const FwdCall& f) {
   const int C = f.a.C;
@@ -1393,8 +1388,8 @@ bool fwd_flat(const FwdCall& f) {
   const FlatPlan pl = flat_plan(f.a.C, sizeof(T), 1, false, 2, kThreads / 32);
   if (pl.rows == 0) return false;
   const int bytes = flat_bytes(pl, f.a.C, 2);
-  static int allowed = 48 * 1024;
-  allow_smem(norm_fwd_long_kernel<T>, bytes, allowed);
+  static SmemOptIn opted;
+  allow_smem(opted, norm_fwd_long_kernel<T>, kRingBudget);
   norm_fwd_long_kernel<T><<<grid_for(f.a.rows, pl.rows, 2), kThreads, bytes, f.s>>>(
       (const T*)f.x.p, (uint32_t)f.a.rows, f.a.C, f.vec(), f.a.eps, f.a.layer, (T*)f.y, f.stats, kept_of(f.k), pl);
   return true;
@@ -1473,8 +1468,8 @@ void bwd_staged(const BwdCall& b) {
     return;
   }
   const auto kernel = norm_bwd_staged_kernel<T, G, UPT, DEPTH, CTAS, LAYER, KEPT>;
-  static bool ready = false;
-  if (!ready) ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) == cudaSuccess;
+  static SmemOptIn opted;
+  allow_smem(opted, kernel, BYTES);
   kernel<<<grid, NT, BYTES, b.s>>>(view_of(b.dy), view_of(b.x), kept_of(b.k), (uint32_t)b.a.rows, b.a.C, b.vec(),
                                    b.stats, (T*)b.dx, b.part, b.dw, b.db);
   b.finish(grid);
@@ -1505,8 +1500,8 @@ void bwd_group(const BwdCall& b) {
     return;
   }
   const auto kernel = norm_bwd_flat_kernel<T, G, UPT, R, KEPT>;
-  static bool ready = false;
-  if (!ready) ready = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) == cudaSuccess;
+  static SmemOptIn opted;
+  allow_smem(opted, kernel, BYTES);
   kernel<<<grid, B::NT, BYTES, b.s>>>((const T*)b.dy.p, (const T*)b.x.p, kept_of(b.k), (uint32_t)b.a.rows, b.a.C,
                                       b.vec(), b.a.layer, b.stats, (T*)b.dx, b.part, b.dw, b.db);
   b.finish(grid);
@@ -1522,8 +1517,8 @@ bool bwd_long(const BwdCall& b) {
     return true;
   }
   const int bytes = flat_bytes(pl, b.a.C, 1);
-  static int allowed = 48 * 1024;
-  allow_smem(norm_bwd_long_kernel<T, NT, E, KEPT>, bytes, allowed);
+  static SmemOptIn opted;
+  allow_smem(opted, norm_bwd_long_kernel<T, NT, E, KEPT>, kRingBudget);
   norm_bwd_long_kernel<T, NT, E, KEPT><<<grid, NT, bytes, b.s>>>(
       (const T*)b.dy.p, (const T*)b.x.p, kept_of(b.k), (uint32_t)b.a.rows, b.a.C, b.vec(), b.a.layer, b.stats, (T*)b.dx,
       b.part, b.dw, b.db, pl);

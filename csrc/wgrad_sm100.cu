@@ -22,6 +22,7 @@
 #include "kept8.cuh"
 #include "launchers.h"
 #include "sm100.cuh"
+#include "smem_opt_in.h"
 
 namespace pan {
 namespace wgrad {
@@ -321,12 +322,8 @@ const char* launch_wgrad(const WgradPlan& pl, const void* dy, long long lddy, co
     else maps.part = maps.d;
   }
   if (err != nullptr) return err;
-  static bool ready = false;
-  if (!ready) {
-    if (cudaFuncSetAttribute(wgrad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess)
-      return "wgrad: cannot set the dynamic shared memory size";
-    ready = true;
-  }
+  static SmemOptIn opted;
+  if (!allow_smem(opted, wgrad_kernel, SMEM_BYTES)) return "wgrad: cannot set the dynamic shared memory size";
   const int pairs = gemm::num_sms() / 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * (p.items < pairs ? p.items : pairs), 1, 1);

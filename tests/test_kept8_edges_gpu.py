@@ -174,3 +174,37 @@ def test_swiglu_ffn_at_odd_addresses():
         assert torch.equal(a, b)
     with torch.no_grad():
         assert torch.equal(kept8_swiglu_ffn(odd_copy(x), w1, w3, w2), want[0])
+
+
+def test_norms_of_many_widths_from_several_threads():
+    import threading
+    widths = [1101, 1535, 2901, 3501, 5001, 7001, 8191, 12001]
+    data = {}
+    for C in widths:
+        x = R.activations(64, C, seed=C, device="cuda").requires_grad_(True)
+        w = torch.linspace(0.5, 1.5, C, device="cuda").requires_grad_(True)
+        data[C] = (x, w, torch.ones_like(x))
+
+    def run(C):
+        x, w, dy = data[C]
+        y = rms_norm(x, w, kept8=True)
+        return (y, *torch.autograd.grad(y, (x, w), dy))
+    failed, got = [], {}
+
+    def work(i):
+        try:
+            for C in widths[i:] + widths[:i]:
+                got[i, C] = run(C)
+        except Exception as e:  # noqa: BLE001 - reported below
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(widths))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for C in widths:
+        want = run(C)
+        for i in range(len(widths)):
+            assert all(torch.equal(a, b) for a, b in zip(got[i, C], want)), (i, C)
