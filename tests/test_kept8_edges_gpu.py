@@ -208,3 +208,48 @@ def test_norms_of_many_widths_from_several_threads():
         want = run(C)
         for i in range(len(widths)):
             assert all(torch.equal(a, b) for a, b in zip(got[i, C], want)), (i, C)
+
+
+@pytest.mark.parametrize("C", [128, 1001], ids=["aligned", "odd"])
+def test_swiglu_of_fp32_is_fp32_arithmetic(C):
+    """h, dgate and dvalue to a few fp32 roundings of themselves, far into the sigmoid's tails too."""
+    rows = 60
+    gate = torch.empty(rows, C, device="cuda")
+    # whole numbers times a power of two, at most 127 of them: what the store reads back is the gate itself
+    step = torch.tensor([2.0 ** (-r % 9 - 6) for r in range(rows)], device="cuda")[:, None]
+    gen = torch.Generator().manual_seed(C)
+    gate.copy_(torch.randint(-110, 100, (rows, C), generator=gen))
+    gate[:, ::32] = 64
+    gate *= step * 32
+    gate[:6] = gate[:6] / gate[:6].abs().amax() * 86  # no longer whole numbers: the forward's only
+    value = torch.randn(rows, C, generator=gen).cuda()
+    gate.requires_grad_(True), value.requires_grad_(True)
+    dh = torch.randn(rows, C, generator=gen).cuda()
+    h = kept8_swiglu(gate, value)
+    dg, dv = torch.autograd.grad(h, (gate, value), dh)
+    ref = R.swiglu(gate, value, dh)
+    g, kv = R.kept_values(gate), R.kept_values(value)
+    assert float(d(gate).min()) < -80 and bool((g[6:] == d(gate)[6:]).all())
+    # exp good to 2 ulp (4 roundings), a sum, a quotient, four products; terms that vanish below the smallest normal
+    tiny = 2.0 ** -126
+    R.check(h, ref["h"], torch.float32, 14 * R.F32 * ref["h"].abs() + tiny, "h")
+    R.check(dv, ref["dvalue"], torch.float32, 14 * R.F32 * ref["dvalue"].abs() + tiny, "dvalue")
+    s = torch.sigmoid(g)
+    terms = (d(dh) * kv * s).abs() * (1 + g.abs() * torch.sigmoid(-g))  # what the slope adds up
+    R.check(dg, ref["dgate"], torch.float32, 18 * R.F32 * terms + tiny, "dgate")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_swiglu_at_the_ends_of_the_range(dtype):
+    g = torch.tensor([-1e30, -1000.0, -120.0, -104.0, -89.0, -88.0, -87.5, 0.0, -0.0, 88.0, 89.0, 120.0, 1e30], device="cuda")
+    gate = torch.zeros(len(g), 64, device="cuda", dtype=dtype)
+    gate[:, 0] = g.to(dtype)  # a block of its own: kept to half a step
+    value, dh = torch.ones_like(gate), torch.ones_like(gate)
+    gate.requires_grad_(True), value.requires_grad_(True)
+    h = kept8_swiglu(gate, value)
+    dg, dv = torch.autograd.grad(h, (gate, value), dh)
+    ref = R.swiglu(gate, value, dh)
+    # results below 2^-119 may vanish: the sigmoid's smallest normal value times |g| < 128
+    for t, name in ((h, "h"), (dg, "dgate"), (dv, "dvalue")):
+        assert bool(torch.isfinite(t).all()), name
+        R.check(t, ref[name], dtype, 32 * R.F32 * ref[name].abs() + 2.0 ** -119, name)
