@@ -94,8 +94,9 @@ def _keep_cpu(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     v = v.view(rows, v.shape[1] // BLOCK, BLOCK)
     top = v.abs().amax(-1)
     finite = torch.isfinite(top)
-    # frexp: top = m * 2^e with m in [1/2, 1), so floor(log2(top)) = e - 1
+    # frexp: top = m * 2^e with m in [1/2, 1), so floor(log2(top)) = e - 1; of 0 it gives e = 0
     byte = (torch.frexp(torch.where(finite, top, torch.ones_like(top)))[1] + 126).clamp(7, 254)
+    byte = torch.where(top == 0, torch.full_like(byte, 7), byte)
     step = torch.ldexp(torch.ones_like(top), byte - 133)
     codes = torch.round(v / step.unsqueeze(-1)).clamp(-127, 127)
     codes = torch.where(finite.unsqueeze(-1), codes, torch.zeros_like(codes)).to(torch.int8).flatten(1)

@@ -199,3 +199,11 @@ def refuses_second_derivatives(dtype, device):
 def test_second_derivatives_are_refused(dtype):
     """The backward reads statistics and codes that carry no graph, so what it returns must not be differentiated."""
     refuses_second_derivatives(dtype, "cpu")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+def test_scale_bytes(dtype):
+    """Exponent of the block's largest value, 7 for blocks of zeros and subnormals, 255 for non-finite ones, 127 for padding."""
+    x = torch.zeros(1, 6 * 32, dtype=dtype)
+    x[0, 32], x[0, 64 + 31], x[0, 96], x[0, 128], x[0, 160] = 1.0, -3.0, 2.0 ** -130, float("inf"), 2.0 ** -126
+    assert keep8(x).scales.tolist() == [[7, 127, 128, 7, 255, 7, 127, 127]]

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import kept8_ref as R
-from pan2_b200.ops.kept8 import kept8_linear, kept8_swiglu, kept8_swiglu_ffn
+from pan2_b200.ops.kept8 import keep8, kept8_linear, kept8_swiglu, kept8_swiglu_ffn
 from pan2_b200.ops.norm import layer_norm, rms_norm
 
 pytestmark = pytest.mark.gpu
@@ -253,3 +253,12 @@ def test_swiglu_at_the_ends_of_the_range(dtype):
     for t, name in ((h, "h"), (dg, "dgate"), (dv, "dvalue")):
         assert bool(torch.isfinite(t).all()), name
         R.check(t, ref[name], dtype, 32 * R.F32 * ref[name].abs() + 2.0 ** -119, name)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("C", [96, 97, 104], ids=["aligned", "odd", "short block"])
+def test_blocks_of_zeros_hold_the_same_bytes_as_on_the_cpu(C, dtype):
+    x = R.activations(70, C, dtype=dtype)
+    x[::3, :32], x[1::3, 64:], x[5] = 0, 0, 0
+    cpu, gpu = keep8(x), keep8(x.cuda())
+    assert torch.equal(cpu.codes, gpu.codes.cpu()) and torch.equal(cpu.scales, gpu.scales.cpu())
