@@ -442,7 +442,7 @@ torch::Tensor norm(torch::Tensor x, OptTensor w, OptTensor b, double eps, bool l
   if (w.has_value() && !w->is_contiguous()) w = w->contiguous();
   if (b.has_value() && !b->is_contiguous()) b = b->contiguous();
   const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(w) || wants_grad(b));
-  return NormNode::apply(x, w, b, eps, layer, kept && (x.requires_grad() || wants_grad(w)), grad);
+  return NormNode::apply(x, w, b, eps, layer, kept, grad);
 }
 
 // x, w, b: bf16 or fp32; computed in bf16.

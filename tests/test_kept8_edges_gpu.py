@@ -262,3 +262,91 @@ def test_blocks_of_zeros_hold_the_same_bytes_as_on_the_cpu(C, dtype):
     x[::3, :32], x[1::3, 64:], x[5] = 0, 0, 0
     cpu, gpu = keep8(x), keep8(x.cuda())
     assert torch.equal(cpu.codes, gpu.codes.cpu()) and torch.equal(cpu.scales, gpu.scales.cpu())
+
+
+@pytest.mark.parametrize("rows,K,N", [(32769, 64, 72), (70001, 33, 20), (65536, 520, 264)])
+def test_linear_of_more_rows_than_are_reloaded_at_once(rows, K, N):
+    """The weight gradient reloads 32768 rows at a time and adds the later ones in fp32."""
+    for w_dtype in (torch.bfloat16, torch.float32):
+        x = bf16(rows, K, seed=rows)
+        w = bf16(N, K, seed=1).to(w_dtype).requires_grad_(True)
+        dy = bf16(rows, N, seed=2)
+        (dw,) = torch.autograd.grad(kept8_linear(x, w), w, dy)
+        k64 = R.kept_values(x)
+        R.check(dw, d(dy).t() @ k64, w_dtype, product_terms(d(dy).t(), k64), "dw")
+
+
+def test_linear_repeats_bit_for_bit():
+    """On a busy GPU, on another stream, after other work: sums run in one order."""
+    x, w, b = bf16(4099, 1024, seed=1), bf16(1544, 1024, seed=2, scale=0.03), bf16(1544, seed=3)
+    dy = bf16(4099, 1544, seed=4)
+    args = [t.requires_grad_(True) for t in (x, w, b)]
+
+    def run():
+        y = kept8_linear(*args)
+        return (y.detach(), *torch.autograd.grad(y, args, dy))
+    first, junk, side = run(), torch.empty(1 << 26, device="cuda"), torch.cuda.Stream()
+    for i in range(12):
+        if i % 3 == 1:
+            junk.normal_()
+        if i % 3 == 2:
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                got = run()
+            torch.cuda.current_stream().wait_stream(side)
+        else:
+            got = run()
+        assert all(torch.equal(p, q) for p, q in zip(first, got)), i
+
+
+def test_linear_of_views():
+    base, wide_w, dys = bf16(4, 50, 3, 96, seed=1), bf16(80, 120, seed=2, scale=0.1), bf16(400, 160, seed=3)
+    inputs = {"aligned columns": base[..., 8:72], "odd columns": base[..., 3:67], "odd width": base[..., 5:38],
+              "middle index": base[:, :, 1, :64], "transposed": base.transpose(0, 2)[..., :64],
+              "three levels": base[::2, ::3, ::2, :64], "last dim strided": base[..., ::2],
+              "expanded": base[:1, :, :, :64].expand(3, -1, -1, -1), "odd address": odd_copy(base[..., :64], 5),
+              "one row": base[0, 0, 0, :64]}
+    for name, x in inputs.items():
+        K, rows = x.shape[-1], x.numel() // x.shape[-1]
+        weights = {"columns": wide_w[:40, 8:8 + K], "odd columns": wide_w[:40, 1:1 + K],
+                   "transposed": bf16(K, 40, seed=5, scale=0.1).t(), "odd address": odd_copy(wide_w[:33, :K])}
+        for w_name, w in weights.items():
+            N = w.shape[0]
+            dy = dys[:, 3:3 + N].repeat(3, 1)[:rows].reshape(*x.shape[:-1], N)
+
+            def run(x, w, dy):
+                x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+                y = kept8_linear(x, w)
+                return (y, *torch.autograd.grad(y, (x, w), dy))
+            want = run(x.contiguous(), w.contiguous(), dy.contiguous())
+            for a, b in zip(want, run(x, w, dy)):
+                assert a.shape == b.shape and torch.equal(a, b), (name, w_name)
+
+
+NORM_FORMS = [(50, 1024), (50, 384), (50, 12288), (50, 77), (50, 1101), (50, 7001), (9, 20001), (0, 64)]
+
+
+@pytest.mark.parametrize("rows,C", NORM_FORMS + [(40, -300), (40, -1500), (40, -9000)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("kept", [False, True], ids=["exact", "kept8"])
+def test_norm_gradients_one_at_a_time(rows, C, dtype, kept):
+    """Any subset of the gradients is the same as in all of them; a negative width is a view at an odd address."""
+    x = R.activations(rows, abs(C) + 1, seed=1, dtype=dtype, device="cuda")
+    x = x[:, :C].contiguous() if C > 0 else x[:, 1:]
+    C = abs(C)
+    w, b = (torch.linspace(lo, lo + 1, C, device="cuda").to(dtype) for lo in (0.5, -0.5))
+    dy = torch.randn(rows, C, generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+
+    def run(*need):
+        args = [t.detach().requires_grad_(n) for t, n in zip((x, w, b), need)]
+        y = layer_norm(*args, kept8=kept)
+        wrt = [a for a in args if a.requires_grad]
+        grads = iter(torch.autograd.grad(y, wrt, dy) if wrt else ())
+        return y, [next(grads) if n else None for n in need]
+    y, full = run(True, True, True)
+    for mask in range(7):
+        need = tuple(bool(mask >> i & 1) for i in range(3))
+        z, some = run(*need)
+        assert torch.equal(y, z), need
+        for a, c in zip(full, some):
+            assert c is None or torch.equal(a, c), need
