@@ -1366,7 +1366,6 @@ bool fwd_flat(const FwdCall& f) {
   const int C = f.a.C;
   constexpr bool B16 = sizeof(T) == 2;
   constexpr int R = B16 ? 4 : 2;  // batches of about 16 KB
-  if (C <= 64) return fwd_group<T, 8, 2, R>(f), true;
 #define GROUP(G) return fwd_group<T, G, 2, R>(f), true
 #define THIRDS(G) if constexpr (B16) if (C <= G * 12) return fwd_group<T, G, 3, 2>(f), true
   if (C <= 64) GROUP(8);

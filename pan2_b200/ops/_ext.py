@@ -34,7 +34,7 @@ def ext():
 # nodes' backwards (norm, linear8, swiglu8) are not calls of a binding and not counted
 KERNELS_PER_CALL = {
     "ln_modulate_bwd": 2, "gate_bwd": 2, "mse_fwd": 2, "attn_bwd": 3, "error_flag": 0, "linear8": 2,
-    "linear8_weight_grad": 2,
+    "linear8_weight_grad": 2, "gemm_operand": 0,  # a copy only where the tensor cannot be read as it lies
 }
 _COUNTING = {"on": False, "launches": 0, "by_name": {}}
 
