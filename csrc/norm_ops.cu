@@ -13,9 +13,11 @@
 // registers, and one partial row of dw / db per CTA goes to scratch, which a second kernel adds up in order (no
 // atomics: the same bits every time).  Four forms:
 //   staged   (C % 8 == 0, 16-byte aligned rows, C <= 16384)  8-column fragments through rings in shared memory
-//   flat     (contiguous rows of other widths, C <= 8192)    batches of rows as runs of bytes (flat.cuh): groups, or warps (long rows)
+//   flat     (contiguous rows of other widths)               batches of rows as runs of bytes (flat.cuh): groups, or warps (long rows);
+//                                                            backward to 8192 columns, forward while two stages fit (14065 fp32, 18753 bf16)
 //   single   (other views, C <= 8192)                        one column at a time, straight from memory
-//   wide     (wider rows)                                    CTA per row, the row swept from memory
+//   wide     (wider rows)                                    CTA per row, the row swept from memory: 6000 x 16001 backward 0.1 (bf16,
+//                                                            kept) to 0.26 (fp32) of the copy rate
 // Groups of up to a warp reduce by shuffles, larger ones through shared memory.
 #include "flat.cuh"
 #include "kept8.cuh"
@@ -508,7 +510,7 @@ __global__ void __launch_bounds__(threads_of(G), CTAS)
 // A batch is GROUPS * R neighbouring rows, one run of bytes; the next two arrive while one is worked on (with one, the kernel
 // waited for memory at 35 % of its bandwidth).  Fragment i of thread t are the 4 columns from 4 (t + i G) on: eight lanes
 // hold a block of the codes.  Results take the place of the input and leave as one run.  What bounds it is instruction
-// issue: single elements are read, converted and masked (48 instructions an element in the forward of width 631), so
+// issue: single elements are read, converted and masked (50 instructions an element in the kept forward of width 631), so
 // bf16 groups are sized for few idle lanes: 100 M elements, layer norm, kept forward / kept backward, two fragments of
 // twice the threads and then three a thread: width 333 269 / 250 and 210 / 182 us, 631 268 / 272 and 215 / 192, 77 291 / 249
 // and 213 / 191.  Packed fp32 pairs cost more in moves than they save here (631: 226 / 217), and so does a branch for
@@ -1573,7 +1575,8 @@ void bwd_wide(const BwdCall& b) {
   b.finish(parts);
 }
 
-// THIRDS as in the forward, bf16 only
+// THIRDS as in the forward, bf16 only.  Fp32 rows past 8192 columns leave room for one stage beside an exact input, so nothing is
+// copied ahead (6000 x 16384 265 us, 0.69 of the copy rate), and for two beside codes (241 us, 0.57).
 template <typename T, bool LAYER, bool KEPT>
 void bwd_staged_any(const BwdCall& b) {
   const int C = b.a.C;
