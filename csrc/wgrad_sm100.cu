@@ -132,7 +132,7 @@ wgrad_kernel(const __grid_constant__ Params p, const __grid_constant__ Maps maps
         const Item it = item_of(p, w);
         const int n0 = it.nt * TILE + crank * HALF, k0 = it.kt * TILE + crank * HALF;
         for (int st = it.s0; st < it.s1 && !s_abort; ++st) {
-          if (!mbar_wait(empty_bar(stage), phase ^ 1, 41)) { s_abort = 1; break; }
+          if (!mbar_wait(empty_bar(stage), phase ^ 1, 61)) { s_abort = 1; break; }
           const uint32_t fb = mapa_shared(full_bar(stage), 0);
           if (crank == 0) mbar_expect_tx(full_bar(stage), 2 * (A_STAGE + B_STAGE));
           const uint32_t sa = smem_u32(smem_a + stage * A_STAGE), sb = smem_u32(smem_b + stage * B_STAGE);
@@ -151,13 +151,13 @@ wgrad_kernel(const __grid_constant__ Params p, const __grid_constant__ Maps maps
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       for (int w = item0; w < p.items && !s_abort; w += item_step) {
-        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1, 42)) { s_abort = 1; break; }
+        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1, 62)) { s_abort = 1; break; }
         tc_fence_after();
         const Item it = item_of(p, w);
         const uint32_t d_tmem = tmem_base + acc * TILE;
         bool ok = true;
         for (int st = it.s0; st < it.s1; ++st) {
-          if (!mbar_wait(full_bar(stage), phase, 43)) { ok = false; break; }
+          if (!mbar_wait(full_bar(stage), phase, 63)) { ok = false; break; }
           tc_fence_after();
           const uint32_t sa = smem_u32(smem_a + stage * A_STAGE), sb = smem_u32(smem_b + stage * B_STAGE);
 #pragma unroll
@@ -187,7 +187,7 @@ wgrad_kernel(const __grid_constant__ Params p, const __grid_constant__ Maps maps
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int w = item0; w < p.items && !s_abort; w += item_step) {
-      if (!mbar_wait(tfull_bar(acc), acc_phase, 44)) { s_abort = 1; break; }
+      if (!mbar_wait(tfull_bar(acc), acc_phase, 64)) { s_abort = 1; break; }
       tc_fence_after();
       const Item it = item_of(p, w);
       const bool fp32 = it.piece >= 0 || p.d_fp32;
